@@ -44,6 +44,7 @@ OPT_DEFAULTS = {OPT_DECODE_XCD_HANDOVERS: 1, OPT_DECODE_XCD_QKV: 1, OPT_DECODE_P
                 OPT_PREFILL_WIDE_TILES: 1, OPT_PREFILL_FUSED_FFN: 1, OPT_PREFILL_MFMA_ATTENTION: 1, OPT_DECODE_CALIBRATE: 1, OPT_PREFILL_ROOM: 0,
                 OPT_DECODE_RESIDENT: 1}
 TOKENIZER_SENTENCEPIECE, TOKENIZER_BPE = 0, 1
+F32, F16 = 0, 1  # element types of activations
 
 
 class LppConfig(C.Structure):
@@ -68,6 +69,12 @@ class LppRunResult(C.Structure):
 class LppKernelTime(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("launches_per_token", C.c_int), ("avg_ms", C.c_double),
                 ("bytes_per_launch", C.c_double)]
+
+
+class LppKv4Shape(C.Structure):
+    """lpp_kv4_shape: what a cache of 4 bits has room for."""
+    _fields_ = [("n_layers", C.c_int), ("n_seqs", C.c_int), ("n_kv_heads", C.c_int), ("seq_len", C.c_int),
+                ("head_size", C.c_int)]
 
 
 class LppError(RuntimeError):
@@ -136,6 +143,14 @@ SIGNATURES = {
     "lpp_tokenizer_info": (_i, [_vp, _ip, _ip, _ip]),
     "lpp_tokenizer_encode": (_i, [_vp, C.c_char_p, _vp, _i, _ip]),
     "lpp_tokenizer_decode": (_i, [_vp, _i, C.c_char_p, _sz]),
+    # E. packed prompts and the cache of 4 bits
+    "lpp_prompt_attention": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "lpp_kv4_bytes": (_i, [C.POINTER(LppKv4Shape), C.POINTER(_sz)]),
+    "lpp_kv4_store": (_i, [_vp, C.POINTER(LppKv4Shape), _i, _vp, _vp, _i, _i, _vp, _i, _vp]),
+    "lpp_kv4_load": (_i, [_vp, _vp, _vp, C.POINTER(LppKv4Shape), _i, _i, _i]),
+    "lpp_kv4_attention_workspace": (_i, [C.POINTER(LppKv4Shape), _i, _i, C.POINTER(_sz)]),
+    "lpp_kv4_attention": (_i, [_vp, _vp, _vp, C.POINTER(LppKv4Shape), _i, _i, _i, _vp, _vp, _vp, _sz]),
+    "lpp_kv4_evict": (_i, [_vp, C.POINTER(LppKv4Shape), _i, _vp, _vp, _vp, _vp, C.POINTER(LppKv4Shape), _i, _vp, _vp, _i, _i]),
     # C. runtime
     "lpp_last_error": (C.c_char_p, []),
     "lpp_version": (C.c_char_p, []),

@@ -1,0 +1,93 @@
+// kv4.hpp -- the cache of 4 bits: where its parts lie, what a word of codes
+// stands for, and the checks its entry points share.
+#pragma once
+
+#include "lpp_device.hpp"
+#include "lpp_internal.hpp"
+
+namespace lpp {
+
+constexpr int kKv4Group = 32;             // values that share a scale
+constexpr int kKv4MaxSeqLen = 1 << 24;    // a head's rows stay within 31 bits of bytes
+constexpr int kMaxSharedHeads = 16;       // query heads to a KV head
+
+// One layer of a cache: rows of its four parts, [sequence][KV head][position].
+struct Kv4Layer {
+    uint32_t* codes[2];   // K, V: head_size / 8 words a row
+    uint32_t* scales[2];  // head_size / 32 words a row: scale in the low half, lowest value in the high half
+};
+
+inline size_t kv4_layer_rows(const lpp_kv4_shape& s) { return static_cast<size_t>(s.n_seqs) * s.n_kv_heads * s.seq_len; }
+
+inline Kv4Layer kv4_layer(const void* cache, const lpp_kv4_shape& s, int layer) {
+    const size_t rows = kv4_layer_rows(s) * s.n_layers, before = kv4_layer_rows(s) * layer;
+    const size_t code_words = s.head_size / 8, scale_words = s.head_size / kKv4Group;
+    uint32_t* base = const_cast<uint32_t*>(static_cast<const uint32_t*>(cache));
+    Kv4Layer l;
+    l.codes[0] = base + before * code_words;
+    l.codes[1] = base + (rows + before) * code_words;
+    l.scales[0] = base + 2 * rows * code_words + before * scale_words;
+    l.scales[1] = base + 2 * rows * code_words + (rows + before) * scale_words;
+    return l;
+}
+
+inline size_t kv4_bytes(const lpp_kv4_shape& s) { return kv4_layer_rows(s) * s.n_layers * s.head_size / 4 * 5; }
+
+// (the product of the counts fits 40 bits, and so every offset 64)
+inline lpp_status kv4_check_shape(const char* who, const lpp_kv4_shape* s) {
+    LPP_REQUIRE(s != nullptr, "%s: null shape", who);
+    LPP_REQUIRE(s->n_layers > 0 && s->n_seqs > 0 && s->n_kv_heads > 0 && s->seq_len > 0,
+                "%s: n_layers = %d, n_seqs = %d, n_kv_heads = %d, seq_len = %d", who, s->n_layers, s->n_seqs, s->n_kv_heads, s->seq_len);
+    LPP_REQUIRE(s->head_size == 64 || s->head_size == 128, "%s: head_size = %d is neither 64 nor 128", who, s->head_size);
+    LPP_REQUIRE(s->seq_len <= kKv4MaxSeqLen, "%s: seq_len = %d beyond %d", who, s->seq_len, kKv4MaxSeqLen);
+    const double rows = static_cast<double>(s->n_layers) * s->n_seqs * s->n_kv_heads * s->seq_len;
+    LPP_REQUIRE(rows <= 1099511627776.0, "%s: %.0f rows are beyond 2^40", who, rows);
+    return LPP_OK;
+}
+inline lpp_status kv4_check_cache(const char* who, const void* cache, const lpp_kv4_shape* s, int layer) {
+    LPP_TRY(kv4_check_shape(who, s));
+    LPP_REQUIRE(cache != nullptr, "%s: null cache", who);
+    LPP_REQUIRE(reinterpret_cast<uintptr_t>(cache) % 16 == 0, "%s: the cache is not 16-byte aligned", who);
+    LPP_REQUIRE(layer >= 0 && layer < s->n_layers, "%s: layer = %d outside [0, %d)", who, layer, s->n_layers);
+    return LPP_OK;
+}
+
+inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
+namespace dev {
+
+// The eight binary16 numbers that a word of codes stands for.  A code in the last bits of a half whose exponent is that of
+// 1024 is 1024 + code, so a pair costs one and-or, one (exact) subtraction and one fused multiply-add, the one rounding.
+__device__ __forceinline__ half8_t kv4_values(uint32_t codes, uint32_t scale_and_low) {
+    const half2_t both = __builtin_bit_cast(half2_t, scale_and_low);
+    const half2_t scale = {both[0], both[0]}, low = {both[1], both[1]}, base = {static_cast<half_t>(1024.0f), static_cast<half_t>(1024.0f)};
+    half8_t v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t bits = ((codes >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
+        const half2_t pair = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, bits) - base, scale, low);
+        v[2 * i] = pair[0];
+        v[2 * i + 1] = pair[1];
+    }
+    return v;
+}
+
+// The sequence that has packed row `row`: the number of sequences that end at or before it (n_seqs: none has it).  `ends`
+// does not decrease.  All lanes of the wavefront call it with the same row and look at 64 ends at a time.
+__device__ __forceinline__ int sequence_of_row(const int* __restrict__ ends, int n_seqs, int row) {
+    int before = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += kWave) {
+        const int s = s0 + lane_id();
+        const bool ended = s < n_seqs && ends[s] <= row;
+        const int here = __popcll(__builtin_amdgcn_ballot_w64(ended));
+        before += here;
+        if (here < kWave) break;
+    }
+    return before;
+}
+
+}  // namespace dev
+}  // namespace lpp

@@ -1,0 +1,165 @@
+"""Section E of include/lpp.h without a GPU: sizes, and every refusal (a call that is refused does no device work)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import kv4_oracle as ko
+from lighterpp_amd import capi
+from lighterpp_amd.capi import LppKv4Shape as Shape
+
+P = 1 << 20  # an address that is never touched
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return capi.load()
+
+
+def refused(lib, status, word):
+    assert status == capi.LPP_ERR_INVALID_ARG
+    assert word in lib.lpp_last_error(), lib.lpp_last_error()
+
+
+def test_bytes(lib):
+    n = C.c_size_t()
+    for dims in [(1, 1, 1, 1, 64), (3, 2, 8, 100, 128), (32, 64, 8, 131072, 128)]:
+        capi.check(lib.lpp_kv4_bytes(Shape(*dims), C.byref(n)))
+        assert n.value == int(np.prod(dims, dtype=np.int64)) * 5 // 4
+    assert ko.Cache(3, 2, 8, 100, 128).buffer.nbytes == 3 * 2 * 8 * 100 * 128 * 5 // 4
+
+
+@pytest.mark.parametrize("dims", [(0, 1, 1, 1, 64), (1, 0, 1, 1, 64), (1, 1, 0, 1, 64), (1, 1, 1, 0, 64), (1, 1, 1, -5, 64), (1, 1, 1, 8, 48),
+                                  (1, 1, 1, 8, 256), (1, 1, 1, (1 << 24) + 1, 64), (1 << 20, 1 << 20, 1, 8, 64)])
+def test_shapes_refused(lib, dims):
+    n = C.c_size_t()
+    refused(lib, lib.lpp_kv4_bytes(Shape(*dims), C.byref(n)), b"lpp_kv4_bytes")
+    refused(lib, lib.lpp_kv4_store(P, Shape(*dims), 0, P, P, 0, 1 << 20, None, 0, None), b"lpp_kv4_store")
+    refused(lib, lib.lpp_kv4_load(P, P, P, Shape(*dims), 0, 0, 0), b"lpp_kv4_load")
+    refused(lib, lib.lpp_kv4_attention(P, 2 * P, 3 * P, Shape(*dims), 0, 1, 1, P, None, P, 1 << 30), b"lpp_kv4_attention")
+    refused(lib, lib.lpp_kv4_evict(P, Shape(*dims), 0, P, P, P, 3 * P, Shape(*dims), 0, P, P, 1, 0), b"lpp_kv4_evict")
+    refused(lib, lib.lpp_kv4_bytes(None, C.byref(n)), b"null shape")
+    refused(lib, lib.lpp_kv4_bytes(Shape(1, 1, 1, 1, 64), None), b"null output")
+
+
+def test_store_refused(lib):
+    s = Shape(2, 3, 2, 10, 64)
+    call = lambda cache=P, layer=0, k=P, v=P, type=0, stride=128, offsets=None, n=6, starts=None: \
+        lib.lpp_kv4_store(cache, s, layer, k, v, type, stride, offsets, n, starts)  # noqa: E731
+    assert call(n=0) == capi.LPP_OK and call(n=0, k=None, v=None) == capi.LPP_OK
+    refused(lib, call(cache=None), b"null cache")
+    refused(lib, call(cache=P + 4), b"aligned")
+    refused(lib, call(layer=2), b"layer")
+    refused(lib, call(layer=-1), b"layer")
+    refused(lib, call(k=None), b"null pointer")
+    refused(lib, call(v=None), b"null pointer")
+    refused(lib, call(type=2), b"type")
+    refused(lib, call(n=-1), b"n_tokens")
+    refused(lib, call(n=7), b"n_tokens")
+    refused(lib, call(stride=127), b"kv_stride")
+    refused(lib, call(stride=130), b"16 bytes")
+    refused(lib, call(type=1, stride=132), b"16 bytes")
+    refused(lib, call(k=P + 8), b"16 bytes")
+
+
+def test_load_refused(lib):
+    s = Shape(1, 1, 2, 10, 64)
+    call = lambda k=P, v=2 * P, cache=3 * P, layer=0, first=0, count=10: lib.lpp_kv4_load(k, v, cache, s, layer, first, count)  # noqa: E731
+    assert call(count=0) == capi.LPP_OK and call(first=10, count=0) == capi.LPP_OK
+    for bad in [dict(first=-1), dict(count=-1), dict(count=11), dict(first=1), dict(first=11, count=0), dict(first=2 ** 31 - 1, count=2 ** 31 - 1)]:
+        refused(lib, call(**bad), b"positions")
+    refused(lib, call(k=None), b"null pointer")
+    refused(lib, call(v=None), b"null pointer")
+    refused(lib, call(v=2 * P + 2), b"16 bytes")
+    refused(lib, call(k=3 * P + 16), b"overlap")
+    refused(lib, call(k=2 * P), b"overlap")
+    refused(lib, call(cache=None), b"null cache")
+
+
+def test_attention_refused(lib):
+    s = Shape(1, 3, 2, 10, 64)
+    need = C.c_size_t()
+    capi.check(lib.lpp_kv4_attention_workspace(s, 8, 2, C.byref(need)))
+    assert need.value > 0
+    call = lambda out=P, q=2 * P, cache=3 * P, layer=0, heads=8, n_q=2, starts=P, work=4 * P, size=need.value: \
+        lib.lpp_kv4_attention(out, q, cache, s, layer, heads, n_q, starts, None, work, size)  # noqa: E731
+    refused(lib, call(out=None), b"null pointer")
+    refused(lib, call(q=None), b"null pointer")
+    refused(lib, call(starts=None), b"null pointer")
+    refused(lib, call(work=None), b"null pointer")
+    refused(lib, call(cache=None), b"null cache")
+    refused(lib, call(layer=1), b"layer")
+    refused(lib, call(heads=7), b"n_heads")
+    refused(lib, call(heads=0), b"n_heads")
+    refused(lib, call(heads=34), b"query heads")
+    refused(lib, call(n_q=0), b"n_q")
+    refused(lib, call(n_q=11), b"n_q")
+    refused(lib, call(size=need.value - 1), b"workspace")
+    refused(lib, call(out=2 * P + 16), b"overlap")
+    for name in ("out", "q", "work"):
+        refused(lib, call(**{name: 5 * P + 4}), b"16 bytes")
+    refused(lib, lib.lpp_kv4_attention_workspace(s, 8, 2, None), b"null output")
+    refused(lib, lib.lpp_kv4_attention_workspace(s, 5, 2, C.byref(need)), b"n_heads")
+
+
+def test_evict_refused(lib):
+    src, dst = Shape(1, 3, 2, 100, 64), Shape(2, 3, 2, 20, 64)
+    call = lambda cache=P, to=dst, to_layer=0, to_mass=2 * P, to_len=3 * P, kept=4 * P, other=5 * P, layer=0, mass=6 * P, length=7 * P, keep=20, recent=5: \
+        lib.lpp_kv4_evict(cache, to, to_layer, to_mass, to_len, kept, other, src, layer, mass, length, keep, recent)  # noqa: E731
+    for name in ("to_mass", "to_len", "kept", "mass", "length"):
+        refused(lib, call(**{name: None}), b"null pointer")
+    for name in ("cache", "other"):
+        refused(lib, call(**{name: None}), b"null cache")
+        refused(lib, call(**{name: 8 * P + 8}), b"aligned")
+    refused(lib, call(to_layer=2), b"layer")
+    refused(lib, call(layer=1), b"layer")
+    refused(lib, call(keep=21), b"keep")
+    refused(lib, call(keep=0, recent=0), b"keep")
+    refused(lib, call(keep=5, recent=6), b"keep")
+    refused(lib, call(recent=-1), b"keep")
+    for other in (Shape(1, 2, 2, 20, 64), Shape(1, 3, 1, 20, 64), Shape(1, 3, 2, 20, 128)):
+        refused(lib, call(to=other), b"caches are of")
+    refused(lib, call(cache=5 * P + 64), b"overlap")
+    refused(lib, call(to_mass=6 * P + 4), b"overlap")
+    refused(lib, call(to_len=7 * P), b"overlap")
+
+
+def test_prompt_refused(lib):
+    call = lambda out=P, q=2 * P, k=3 * P, v=4 * P, type=0, offsets=5 * P, seqs=2, n=8, heads=4, kv=2, hs=64, sq=256, sk=128, so=256: \
+        lib.lpp_prompt_attention(out, q, k, v, type, offsets, seqs, n, heads, kv, hs, sq, sk, so)  # noqa: E731
+    assert call(n=0) == capi.LPP_OK
+    for name in ("out", "q", "k", "v"):
+        refused(lib, call(**{name: None}), b"null pointer")
+        refused(lib, call(**{name: 6 * P + 8}), b"16 bytes")
+    refused(lib, call(type=3), b"type")
+    refused(lib, call(heads=5), b"n_heads")
+    refused(lib, call(kv=0), b"n_heads")
+    refused(lib, call(heads=34, sq=34 * 64, so=34 * 64), b"query heads")
+    refused(lib, call(hs=48), b"head_size")
+    refused(lib, call(n=-1), b"n_tokens")
+    refused(lib, call(seqs=0), b"n_seqs")
+    refused(lib, call(offsets=None), b"n_seqs")
+    for name in ("sq", "so"):
+        refused(lib, call(**{name: 255}), b"strides")
+        refused(lib, call(**{name: 258}), b"16 bytes")
+    refused(lib, call(sk=127), b"strides")
+    refused(lib, call(sk=132), b"16 bytes")
+    refused(lib, call(out=2 * P + 1024), b"overlap")
+    refused(lib, call(out=4 * P - 16), b"overlap")
+
+
+def test_oracle_groups():
+    """The oracle's own rules: ends of the range, constant groups, overflow."""
+    x = np.zeros((1, 64), np.float32)
+    x[0, :32] = np.linspace(-1, 2, 32)
+    x[0, 40] = 3.0
+    codes, scale, low = ko.quantise(x)
+    assert codes[0, 0, 0] == 0 and codes[0, 0, 31] == 15 and codes[0, 1].max() == 15 and codes[0, 1, 0] == 0
+    v = ko.rounded(x).astype(np.float64)
+    assert np.abs(v - x).max() <= 0.5 * 0.2 * (1 + 2.0 ** -10) + 2 * 2.0 ** -10
+    assert np.array_equal(ko.rounded(np.full((1, 32), 0.3, np.float32)), np.full((1, 32), 0.3, np.float16))
+    for bad in (np.inf, -np.inf, np.nan, 32769.0):
+        y = x.copy()
+        y[0, 3] = bad
+        assert np.isnan(ko.rounded(y)[0, :32]).all() and not np.isnan(ko.rounded(y)[0, 32:]).any()
+    assert not np.isnan(ko.rounded(np.array([[32768.0, -32768.0] * 16], np.float32))).any()

@@ -1,0 +1,171 @@
+"""lpp_prompt_attention against 64 bits: ragged and empty sequences, every number of query heads to a KV head, both types, strides, rows that
+belong to no sequence, and what K and V hold outside a row's own positions."""
+import numpy as np
+import pytest
+
+import kv4_oracle as ko
+from lighterpp_amd import capi
+from lighterpp_amd.capi import DeviceBuffer as DB
+
+pytestmark = pytest.mark.gpu
+F, H = np.float32, np.float16
+
+
+@pytest.fixture(scope="module")
+def lib():
+    lib = capi.load()
+    assert capi.device_count() >= 1, "no HIP device visible"
+    capi.check(lib.lpp_init(0))
+    return lib
+
+
+def run(lib, q, k, v, offsets, n_tokens=None, pad=0, seqs=None):
+    """q [rows, heads, hs], k and v [rows, kv_heads, hs] binary16.  `pad`: groups of 8 elements behind every row, which must not change."""
+    rows, heads, hs = q.shape
+    kv = k.shape[1]
+    typ = q.dtype.type
+    extra = 8 * pad
+
+    def padded(x, fill):
+        return np.concatenate([x.reshape(rows, -1), np.full((rows, extra), fill, x.dtype)], 1)
+
+    dq, dk, dv = DB.from_numpy(padded(q, np.nan)), DB.from_numpy(padded(k, np.nan)), DB.from_numpy(padded(v, np.inf))
+    out = np.full((rows, heads * hs + extra), 7.25, typ)
+    dout = DB.from_numpy(out)
+    doff = None if offsets is None else DB.from_numpy(np.array(offsets, np.int32))
+    seqs = (1 if offsets is None else len(offsets) - 1) if seqs is None else seqs
+    capi.check(lib.lpp_prompt_attention(dout.ptr, dq.ptr, dk.ptr, dv.ptr, capi.F32 if typ is F else capi.F16, doff.ptr if doff else None, seqs,
+                                        rows if n_tokens is None else n_tokens, heads, kv, hs, heads * hs + extra, kv * hs + extra, heads * hs + extra))
+    got = dout.to_numpy(typ, out.size).reshape(out.shape)
+    assert np.all(got[:, heads * hs:] == typ(7.25)), "the space between the rows was written"
+    return got[:, :heads * hs].reshape(rows, heads, hs)
+
+
+def inputs(seed, rows, heads, kv, hs, typ, spread=1.0):
+    rng = np.random.default_rng(seed)
+    return ((rng.standard_normal((rows, heads, hs)) * spread).astype(typ), rng.standard_normal((rows, kv, hs)).astype(H),
+            rng.standard_normal((rows, kv, hs)).astype(H))
+
+
+def against(got, q, k, v, spans):
+    """Every sequence's rows against the oracle, the others untouched."""
+    mine = np.zeros(q.shape[0], bool)
+    worst = 0.0
+    for a, b in spans:
+        mine[a:b] = True
+        if a == b:
+            continue
+        want, _, tol = ko.attend_tolerance(q[a:b], k[a:b].transpose(1, 0, 2), v[a:b].transpose(1, 0, 2), [j + 1 for j in range(b - a)],
+                                           binary16=q.dtype.type is H)
+        off = np.abs(got[a:b].astype(np.float64) - want)
+        worst = max(worst, float((off / tol).max()))
+        assert np.all(off <= tol), (a, b, float((off / tol).max()))
+    assert np.all(got[~mine] == q.dtype.type(7.25))
+    return worst
+
+
+LENGTHS = [[1], [2, 0, 1], [31, 32, 33], [63, 65, 1, 0, 128], [257], [5, 0, 0, 300, 130]]
+
+
+@pytest.mark.parametrize("heads,kv,hs", [(2, 2, 64), (8, 2, 64), (8, 1, 64), (16, 1, 128), (6, 2, 128), (3, 3, 128)])
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("lengths", LENGTHS, ids=str)
+def test_lengths(lib, lengths, typ, heads, kv, hs):
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = inputs(sum(lengths) * heads + hs, int(offsets[-1]), heads, kv, hs, typ)
+    got = run(lib, q, k, v, offsets)
+    against(got, q, k, v, list(zip(offsets[:-1], offsets[1:])))
+
+
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("heads,kv,hs,length", [(4, 1, 64, 1100), (5, 1, 128, 700), (4, 4, 128, 1025)])
+def test_one_long_prompt_without_offsets(lib, heads, kv, hs, length, typ):
+    q, k, v = inputs(length, length, heads, kv, hs, typ)
+    against(run(lib, q, k, v, None, pad=1), q, k, v, [(0, length)])
+
+
+@pytest.mark.parametrize("typ", [F, H])
+def test_many_short_sequences(lib, typ):
+    """More sequences than a wavefront looks at in one go, empty ones among them, also first and last."""
+    rng = np.random.default_rng(5)
+    lengths = rng.integers(0, 9, 200)
+    lengths[:3] = lengths[-2:] = 0
+    lengths[64:130] = 0
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = inputs(6, int(offsets[-1]), 4, 2, 64, typ)
+    against(run(lib, q, k, v, offsets), q, k, v, list(zip(offsets[:-1], offsets[1:])))
+
+
+@pytest.mark.parametrize("typ", [F, H])
+def test_rows_outside_every_sequence_and_strides(lib, typ):
+    """The first offset is not 0, the last is not the end; rows have space behind them."""
+    q, k, v = inputs(7, 150, 6, 2, 64, typ)
+    against(run(lib, q, k, v, [3, 40, 40, 141], pad=3), q, k, v, [(3, 40), (40, 141)])
+
+
+@pytest.mark.parametrize("offsets,spans", [([-5, 20, 1000], [(0, 20), (20, 50)]), ([0, 2 ** 31 - 1], [(0, 50)]), ([50, 50, 50], []),
+                                           ([-2 ** 31, -7, 50], [(0, 50)])])
+def test_offsets_outside_are_cut(lib, offsets, spans):
+    q, k, v = inputs(8, 50, 4, 2, 64, F)
+    against(run(lib, q, k, v, offsets), q, k, v, spans)
+
+
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("hs", [64, 128])
+def test_large_scores(lib, typ, hs):
+    """Scores of some hundreds, growing and falling along the sequence: the running maximum moves by a lot."""
+    q, k, v = inputs(9, 300, 4, 1, hs, typ, spread=4.0)
+    k = (k * np.linspace(0.2, 6.0, 300)[:, None, None]).astype(H)
+    k[200:] = (k[200:] * 0.1).astype(H)
+    against(run(lib, q, k, v, [0, 300]), q, k, v, [(0, 300)])
+
+
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("heads,kv,hs", [(4, 4, 64), (8, 1, 64), (6, 2, 128)])
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_nothing_comes_from_positions_a_row_does_not_attend_to(lib, where, bad, heads, kv, hs, typ):
+    """A K or V row of infinities or NaN in the middle of a tile and one at a sequence's end: rows before it and other sequences are as if
+    it were not there, bit for bit; the row's own output and all behind it show it."""
+    offsets = [0, 37, 150, 181]
+    q, k, v = inputs(10, 190, heads, kv, hs, typ)
+    clean = run(lib, q, k, v, offsets)
+    at = {36: 0, 90: 1, 149: 1}
+    x = {"k": k.copy(), "v": v.copy()}
+    for p in at:
+        x[where][p, :, 3] = bad
+    x[where][181:] = bad  # rows of no sequence
+    got = run(lib, q, x["k"], x["v"], offsets)
+    seen = np.zeros(190, bool)
+    for p, s in at.items():
+        seen[p:offsets[s + 1]] = True
+    assert np.array_equal(got[~seen], clean[~seen])
+    if where == "v":
+        assert not np.isfinite(got[seen][:, :, 3]).any()
+        other = np.ones(hs, bool)
+        other[3] = False
+        assert np.array_equal(got[seen][:, :, other], clean[seen][:, :, other])
+    elif np.isnan(bad):
+        assert np.isnan(got[seen]).all()
+
+
+def test_same_bits_twice(lib):
+    q, k, v = inputs(11, 700, 8, 2, 64, F)
+    a, b = run(lib, q, k, v, [0, 100, 700]), run(lib, q, k, v, [0, 100, 700])
+    assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
+def test_rows_far_apart(lib):
+    """Row offsets beyond 2^31 elements: rows of q and out 2^21 elements apart."""
+    rows, heads, kv, hs, stride = 1100, 2, 1, 64, 1 << 21
+    q, k, v = inputs(12, rows, heads, kv, hs, H)
+    dq, dout = DB(rows * stride * 2), DB(rows * stride * 2)
+    dk, dv = DB.from_numpy(k), DB.from_numpy(v)
+    keep = [0, 1, 500, rows - 30, rows - 1]
+    for r in range(rows):
+        dq.upload(q[r], r * stride * 2)
+    capi.check(lib.lpp_prompt_attention(dout.ptr, dq.ptr, dk.ptr, dv.ptr, capi.F16, None, 1, rows, heads, kv, hs, stride, kv * hs, stride))
+    ends = [j + 1 for j in keep]
+    want, _, tol = ko.attend_tolerance(q[keep], k.transpose(1, 0, 2), v.transpose(1, 0, 2), ends, binary16=True)
+    got = np.stack([dout.to_numpy(H, heads * hs, r * stride * 2).reshape(heads, hs) for r in keep]).astype(np.float64)
+    assert np.all(np.abs(got - want) <= tol)
