@@ -7,43 +7,383 @@ namespace {
 
 using namespace dev;
 
-// One wavefront per (row, query head); a lane has one position's score, then head_size / 64 output values.
-template <typename T>
-__global__ __launch_bounds__(kWave) void prompt_kernel(T* __restrict__ out, const T* __restrict__ q, const half_t* __restrict__ k,
-                                                       const half_t* __restrict__ v, const int* __restrict__ offsets, int n_seqs,
-                                                       int n_heads, int shared, int head_size, int q_stride, int kv_stride, int out_stride, float scale) {
-    const int head = blockIdx.x % n_heads, row = blockIdx.x / n_heads, lane = lane_id();
-    int first = 0;
-    if (offsets != nullptr) {
-        const int s = sequence_of_row(offsets + 1, n_seqs, row);
-        if (s >= n_seqs) return;
-        first = max(offsets[s], 0);
-        if (row < first) return;
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+// A workgroup is kR x kP wavefronts: kR own 32 query rows each, (32 / shared) consecutive tokens x the query heads of one KV head, and share
+// the K and V rows of every step of kStep positions; kP take the steps in turn and merge what they have at the end.
+template <int kHs, int kR, int kP, int kStepRows>
+struct Shape {
+    static constexpr int kStep = kStepRows, kRowBytes = 2 * kHs, kPieces = kHs / 8;
+    static constexpr int kHalfBytes = kStep * kRowBytes, kStageBytes = 2 * kHalfBytes;  // K rows, then V rows
+    static constexpr int kRequests = kStageBytes / 1024 / kR;                           // a wavefront's, of a step
+    static constexpr int kStages = 2;
+    static constexpr int kPartFloats = (kHs / 2 + 2) * 64;  // a wavefront's maximum, sum and output
+    static constexpr int kMergeBytes = kP > 1 ? kP * kR * kPartFloats * 4 : 0;
+    static constexpr int kStepBytes = kP * kStages * kStageBytes;
+    static constexpr int kLdsBytes = kStepBytes > kMergeBytes ? kStepBytes : kMergeBytes;
+    static_assert(kStageBytes % (1024 * kR) == 0, "every wavefront makes the same number of requests");
+    static_assert(kLdsBytes <= 160 * 1024, "LDS of a workgroup");
+};
+
+struct PromptJob {
+    void* out;
+    const void* q;
+    const half_t* k;
+    const half_t* v;
+    const int* offsets;
+    int n_seqs, n_tokens, shared, n_kv_heads;
+    int q_stride, kv_stride, out_stride;
+};
+
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int kCount>
+__device__ __forceinline__ void wait_requests() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCount) : "memory");
+}
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr by 1, 2, 4, 8: zero comes in
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+    const int row = lane_id() >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+
+// The sequence that tile `tile` of all sequences' tiles is in, one behind the other, and which of its tiles: the last one first, so that the
+// longest walks of a sequence begin first.  Returns the sequence's rows, 0: there are not as many tiles.
+__device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& tile, int& first_row) {
+    if (job.offsets == nullptr) {
+        first_row = 0;
+        tile = (job.n_tokens + tokens - 1) / tokens - 1 - tile;
+        return tile >= 0 ? job.n_tokens : 0;
     }
-    const T* qv = q + static_cast<size_t>(row) * q_stride + head * head_size;
-    const half_t* kh = k + head / shared * head_size;
-    const half_t* vh = v + head / shared * head_size;
-    float top = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int p0 = first; p0 <= row; p0 += kWave) {
-        const int p = p0 + lane;
-        float score = -INFINITY;
-        if (p <= row) {
-            score = 0.0f;
-            for (int e = 0; e < head_size; ++e) score = fmaf(static_cast<float>(kh[static_cast<size_t>(p) * kv_stride + e]), static_cast<float>(qv[e]), score);
-            score *= scale;
+    const int lane = lane_id();
+    for (int s0 = 0; s0 < job.n_seqs; s0 += kWave) {
+        const int s = s0 + lane;
+        const int begin = s < job.n_seqs ? min(max(job.offsets[s], 0), job.n_tokens) : 0;
+        const int end = s < job.n_seqs ? min(max(job.offsets[s + 1], 0), job.n_tokens) : 0;
+        const int rows = max(end - begin, 0), tiles = (rows + tokens - 1) / tokens;
+        const int upto = wave_inclusive_sum(tiles);
+        const unsigned long long behind = __builtin_amdgcn_ballot_w64(upto > tile);
+        if (behind != 0ull) {
+            const int at = __builtin_ctzll(behind);
+            first_row = __builtin_amdgcn_readlane(begin, at);
+            tile = __builtin_amdgcn_readlane(upto, at) - 1 - tile;
+            return __builtin_amdgcn_readlane(rows, at);
         }
-        const float grown = fmaxf(top, wave_max(score));
-        const float weight = expf(score - grown), correction = top == -INFINITY ? 0.0f : expf(top - grown);
-        top = grown;
-        sum = sum * correction + wave_sum(weight);
-        const int count = min(kWave, row + 1 - p0);
-        for (int d = 0; d < head_size / kWave; ++d) {
-            acc[d] *= correction;
-            for (int j = 0; j < count; ++j)
-                acc[d] = fmaf(__shfl(weight, j), static_cast<float>(vh[static_cast<size_t>(p0 + j) * kv_stride + d * kWave + lane]), acc[d]);
+        tile -= __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return 0;
+}
+
+__device__ __forceinline__ bool has_nonfinite(half8_t v) {
+    const uintx4 u = __builtin_bit_cast(uintx4, v);
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= (u[i] & 0x7FFF7FFFu) + 0x04000400u;  // (the exponent's carry)
+    return (any & 0x80008000u) != 0u;
+}
+
+template <typename T, int kHs, int kR, int kP, int kStepRows>
+__global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) {
+    typedef Shape<kHs, kR, kP, kStepRows> S;
+    constexpr bool kLo = sizeof(T) == 4;  // heads and remainders
+    constexpr int kDTiles = kHs / 32, kKSteps = kHs / 16, kStep = S::kStep, kRowBytes = S::kRowBytes, kPieces = S::kPieces;
+    constexpr int kTiles = kStep / 32;  // tiles of 32 positions in a step
+    extern __shared__ __align__(1024) char lds[];
+    const int lane = lane_id(), wave = wave_index();
+    const int wr = wave % kR, wp = wave / kR;
+    const int r = lane & 31, g = lane >> 5;
+    const int tokens_per_wave = 32 / job.shared, tokens = kR * tokens_per_wave;
+    // (a KV head's workgroups are n_kv_heads apart: with 8 of them, or a divisor, its rows stay in one die's L2 or few)
+    const int kvh = static_cast<int>(blockIdx.x) % job.n_kv_heads;
+    int tile = static_cast<int>(blockIdx.x) / job.n_kv_heads, first_row = 0;
+    const int rows = find_tile(job, tokens, tile, first_row);
+    if (tile < 0 || tile * tokens >= rows) return;
+    // positions count from the sequence's first row
+    const int first_token = tile * tokens, t0 = first_token + wr * tokens_per_wave;
+    const int limit = min(first_token + tokens, rows);                       // the workgroup reads [0, limit)
+    const int wave_limit = t0 < rows ? min(t0 + tokens_per_wave, rows) : 0;  // the wavefront attends to [0, wave_limit)
+    const int my_tok = t0 + r / job.shared, my_head = r % job.shared;
+    const bool valid = my_tok < rows && r < tokens_per_wave * job.shared;
+    const int tok_c = min(my_tok, rows - 1);
+    const int my_limit = min(tok_c, t0 + tokens_per_wave - 1) + 1;  // this lane's row attends to [0, my_limit)
+    const char* kbase = reinterpret_cast<const char*>(job.k + static_cast<size_t>(first_row) * job.kv_stride + kvh * kHs);
+    const char* vbase = reinterpret_cast<const char*>(job.v + static_cast<size_t>(first_row) * job.kv_stride + kvh * kHs);
+    const size_t row_step = static_cast<size_t>(job.kv_stride) * 2;
+
+    char* stages = lds + wp * S::kStages * S::kStageBytes;
+    const unsigned lds_base = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)stages));
+    const int steps = (limit + kStep - 1) / kStep, turns = (steps + kP - 1) / kP;
+    constexpr int kRowsPerLoad = 1024 / kRowBytes, kLoadsPerHalf = S::kHalfBytes / 1024;
+    auto request = [&](int turn) {
+        const int p0 = (turn * kP + wp) * kStep;
+#pragma unroll
+        for (int i = 0; i < S::kRequests; ++i) {
+            const int load = wr + kR * i, in_half = load % kLoadsPerHalf;
+            const bool is_v = load >= kLoadsPerHalf;  // (uniform)
+            const int row = in_half * kRowsPerLoad + lane / kPieces;
+            const int swizzle = is_v ? (kHs == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3)) : (kHs == 64 ? (row >> 1) & 7 : row & 15);
+            const int pos = min(p0 + row, limit - 1);
+            const char* src = (is_v ? vbase : kbase) + static_cast<size_t>(pos) * row_step + 16 * ((lane % kPieces) ^ swizzle);
+            const unsigned at = __builtin_amdgcn_readfirstlane(lds_base + (turn % S::kStages) * S::kStageBytes + load * 1024);
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n" ::"v"(src), "s"(at) : "memory");
+        }
+    };
+    request(0);
+
+    half8_t qh[kKSteps], ql[kLo ? kKSteps : 1];
+    {
+        const T* qrow = static_cast<const T*>(job.q) + static_cast<size_t>(first_row + tok_c) * job.q_stride + (kvh * job.shared + my_head) * kHs + 8 * g;
+#pragma unroll
+        for (int s = 0; s < kKSteps; ++s) {
+            if constexpr (kLo) {
+                const floatx4 a = as_float4(load16(qrow + 16 * s)), b = as_float4(load16(qrow + 16 * s + 4));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float v = e < 4 ? a[e & 3] : b[e & 3];
+                    const half_t h = static_cast<half_t>(v);
+                    qh[s][e] = h;
+                    ql[s][e] = static_cast<half_t>(v - static_cast<float>(h));
+                }
+            } else {
+                qh[s] = as_half8(load16(qrow + 16 * s));
+            }
         }
     }
-    for (int d = 0; d < head_size / kWave; ++d) out[static_cast<size_t>(row) * out_stride + head * head_size + d * kWave + lane] = static_cast<T>(acc[d] / sum);
+    floatx16 o[kDTiles];
+#pragma unroll
+    for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    constexpr float kSlack = 6.0f;
+    const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
+    float top = 0.0f, lsum = 0.0f;  // (the sum over this lane's own positions)
+    bool seen = false;              // the row has attended to something: top is a score
+    float minus_one = -1.0f;
+    asm("" : "+v"(minus_one));
+
+    // where this lane reads its fragments of a tile: K row r, pieces 2 s + g; V rows 4 g + (lane % 16) / 4 of the first
+    // sixteen, dimensions 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) ..
+    int k_at[kKSteps], v_at[kDTiles];
+#pragma unroll
+    for (int s = 0; s < kKSteps; ++s) k_at[s] = r * kRowBytes + 16 * ((2 * s + g) ^ (kHs == 64 ? (r >> 1) & 7 : r & 15));
+    {
+        const int row = 4 * g + ((lane & 15) >> 2);
+#pragma unroll
+        for (int dt = 0; dt < kDTiles; ++dt) {
+            const int piece = 4 * dt + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            v_at[dt] = row * kRowBytes + 16 * (piece ^ (kHs == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3))) + 8 * (lane & 1);
+        }
+    }
+
+    for (int turn = 0; turn < turns; ++turn) {
+        const int p0 = (turn * kP + wp) * kStep;
+        // (the step's rows have landed, and nobody reads the stage the next requests go to any more)
+        wait_requests<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (kR > 1) __syncthreads();
+        if (turn + 1 < turns) request(turn + 1);
+        if (p0 >= wave_limit) continue;
+        const char* stage = stages + (turn % S::kStages) * S::kStageBytes;
+        const char* values = stage + S::kHalfBytes;
+        floatx16 st[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[t][e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kKSteps; ++s) {
+                const half8_t kf = *reinterpret_cast<const half8_t*>(stage + t * 32 * kRowBytes + k_at[s]);
+                st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[s], st[t], 0, 0, 0);
+                if constexpr (kLo) st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[s], st[t], 0, 0, 0);
+            }
+        }
+        const bool partly = p0 + kStep > t0 + 1;  // (uniform) some row of the wavefront does not attend to the whole step
+        if (partly) {
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int pos = p0 + 32 * t + 8 * (e >> 2) + 4 * g + (e & 3);
+                    st[t][e] = pos < my_limit ? st[t][e] : -INFINITY;
+                }
+        }
+        float step_top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) step_top = fmaxf(step_top, st[t][e]);
+        step_top = halves_max(step_top) * scale;
+        if constexpr (kLo) step_top = __builtin_ceilf(step_top);
+        const bool moves = step_top > (seen ? top + kSlack : -INFINITY);
+        if (__builtin_amdgcn_ballot_w64(moves) != 0ull) {  // (uniform)
+            const float to = moves ? step_top : top;
+            const float corr = __builtin_amdgcn_exp2f(seen ? top - to : 0.0f);  // (nothing to rescale before a row's first step)
+            top = to;
+            lsum *= corr;
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= corr;
+            seen = seen || moves;
+        }
+        float step_sum = 0.0f;  // (of its own, so that the running sum is rounded once a step)
+#pragma unroll
+        for (int s2 = 0; s2 < 2 * kTiles; ++s2) {
+            half8_t ph, pl;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float s_0 = st[s2 >> 1][8 * (s2 & 1) + e], s_1 = st[s2 >> 1][8 * (s2 & 1) + e + 1];
+                float p_0 = __builtin_amdgcn_exp2f(fmaf(s_0, scale, -top)), p_1 = __builtin_amdgcn_exp2f(fmaf(s_1, scale, -top));
+                step_sum += p_0 + p_1;
+                // (the packed pair and the factor -1 are hidden from the compiler, which would otherwise round every value a second time to
+                // subtract it)
+                uint32_t packed = __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(p_0), static_cast<half_t>(p_1)});
+                if constexpr (kLo) asm("" : "+v"(packed));
+                const half2_t h = __builtin_bit_cast(half2_t, packed);
+                ph[e] = h[0];
+                ph[e + 1] = h[1];
+                if constexpr (kLo) {
+                    pl[e] = static_cast<half_t>(fmaf(static_cast<float>(h[0]), minus_one, p_0));
+                    pl[e + 1] = static_cast<half_t>(fmaf(static_cast<float>(h[1]), minus_one, p_1));
+                }
+            }
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt) {
+                union {
+                    short4_t part[2];
+                    half8_t whole;
+                } vf;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    vf.part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (__attribute__((address_space(3))) short4_t*)(values + v_at[dt] + (16 * s2 + 8 * j) * kRowBytes));
+                if (partly && __builtin_amdgcn_ballot_w64(has_nonfinite(vf.whole)) != 0ull) {
+                    // (uniform) An infinity or NaN among V rows that some row does not attend to: a weight of zero would not keep it out.  One
+                    // token after the other, with the rows behind it cleared; a lane's output is its own token's.
+                    for (int token = 0; token < tokens_per_wave; ++token) {
+                        const int end = t0 + token + 1 - p0 - 16 * s2 - 4 * g;  // positions 0..3 and 8..11 from here are this lane's
+                        half8_t seen_v = vf.whole;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if ((e & 3) + 8 * (e >> 2) >= end) seen_v[e] = static_cast<half_t>(0.0f);
+                        floatx16 with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, ph, o[dt], 0, 0, 0);
+                        if constexpr (kLo) with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
+                        if (r / job.shared == token) o[dt] = with;
+                    }
+                } else {
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, ph, o[dt], 0, 0, 0);
+                    if constexpr (kLo) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, pl, o[dt], 0, 0, 0);
+                }
+            }
+        }
+        lsum += step_sum;
+    }
+    lsum = halves_sum(lsum);
+    T* out_row = static_cast<T*>(job.out) + static_cast<size_t>(first_row + tok_c) * job.out_stride + (kvh * job.shared + my_head) * kHs + 4 * g;
+    auto store4 = [&](int four, floatx4 v) {
+        const int at = 32 * (four >> 2) + 8 * (four & 3);
+        if constexpr (kLo) {
+            *reinterpret_cast<floatx4*>(out_row + at) = v;
+        } else {
+            half4_t h;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) h[u] = static_cast<half_t>(v[u]);
+            *reinterpret_cast<half4_t*>(out_row + at) = h;
+        }
+    };
+    constexpr int kFours = kHs / 8;
+    auto four_of = [&](int four) { return floatx4{o[four >> 2][4 * (four & 3)], o[four >> 2][4 * (four & 3) + 1], o[four >> 2][4 * (four & 3) + 2], o[four >> 2][4 * (four & 3) + 3]}; };
+    if constexpr (kP == 1) {
+        if (!valid) return;
+        const float inv_sum = 1.0f / lsum;
+#pragma unroll
+        for (int four = 0; four < kFours; ++four) store4(four, four_of(four) * inv_sum);
+    } else {
+        // The wavefronts of a row meet in LDS, lane for lane: each leaves its (maximum, sum, output), and each adds up its share of the
+        // output's pieces of four values in the order of the wavefronts.  Those past the last step have left nothing and are not read.
+        if (!seen) top = -INFINITY;
+        __syncthreads();  // (the stages are free)
+        constexpr int kPart = S::kPartFloats;
+        const int parts = min(steps, kP);
+        float* merge = reinterpret_cast<float*>(lds) + wr * kP * kPart;
+        if (wp < parts) {
+            float* mine = merge + wp * kPart;
+            mine[lane] = top;
+            mine[64 + lane] = lsum;
+#pragma unroll
+            for (int four = 0; four < kFours; ++four) *reinterpret_cast<floatx4*>(mine + 128 + 256 * four + 4 * lane) = four_of(four);
+        }
+        __syncthreads();
+        if (!valid) return;
+        float weight[kP], all_top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kP; ++w) {
+            weight[w] = w < parts ? merge[w * kPart + lane] : -INFINITY;
+            all_top = fmaxf(all_top, weight[w]);
+        }
+        if (all_top == -INFINITY) all_top = 0.0f;  // (no score was a number)
+#pragma unroll
+        for (int w = 0; w < kP; ++w) {
+            weight[w] = __builtin_amdgcn_exp2f(weight[w] - all_top);
+            if (w < parts) total = fmaf(merge[w * kPart + 64 + lane], weight[w], total);
+        }
+        const float inv_sum = 1.0f / total;
+#pragma unroll
+        for (int f = 0; f < kFours / kP; ++f) {
+            const int four = wp + kP * f;
+            floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kP; ++w) {
+                if (w >= parts) break;
+                const floatx4 a = *reinterpret_cast<const floatx4*>(merge + w * kPart + 128 + 256 * four + 4 * lane);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = fmaf(a[u], weight[w], v[u]);
+            }
+            store4(four, v * inv_sum);
+        }
+    }
+}
+
+template <typename T, int kHs, int kR, int kP, int kStepRows>
+lpp_status launch_as(const PromptJob& job, int n_seqs) {
+    constexpr int kLds = Shape<kHs, kR, kP, kStepRows>::kLdsBytes;
+    const auto kernel = &prompt_kernel<T, kHs, kR, kP, kStepRows>;
+    if constexpr (kLds > 64 * 1024) {  // told to the runtime once per device
+        static bool sized[64] = {};
+        int device = 0;
+        LPP_HIP(hipGetDevice(&device));
+        if (device < 0 || device >= 64 || !sized[device]) {
+            LPP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+            if (device >= 0 && device < 64) sized[device] = true;
+        }
+    }
+    // (as many tiles as sequences of any lengths can have)
+    const int tokens = kR * (32 / job.shared);
+    const long long tiles = job.n_tokens / tokens + (n_seqs < job.n_tokens ? n_seqs : job.n_tokens);
+    const long long blocks = tiles * job.n_kv_heads;
+    LPP_REQUIRE(blocks * 64 * kR * kP < (1ll << 32), "lpp_prompt_attention: %d rows of %d KV heads are too many for a launch", job.n_tokens, job.n_kv_heads);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kR * kP), kLds, stream(), job);
+    LPP_CHECK_LAUNCH("prompt_kernel");
+    return LPP_OK;
+}
+
+template <typename T, int kHs>
+lpp_status launch(const PromptJob& job, int n_seqs) {
+    const long long tiles = (static_cast<long long>(job.n_tokens) * job.shared + 31) / 32 * job.n_kv_heads;  // of 32 rows
+    if (tiles <= 2ll * compute_units()) return launch_as<T, kHs, 1, 4, 32>(job, n_seqs);
+    return launch_as<T, kHs, 4, 1, 64>(job, n_seqs);
 }
 
 }  // namespace
@@ -76,18 +416,21 @@ lpp_status lpp_prompt_attention(void* d_out, const void* d_q, const lpp_half* d_
     LPP_REQUIRE(!ranges_overlap(d_out, out_bytes, d_q, q_bytes) && !ranges_overlap(d_out, out_bytes, d_k, kv_bytes) &&
                     !ranges_overlap(d_out, out_bytes, d_v, kv_bytes),
                 "lpp_prompt_attention: d_out overlaps an input");
-    const float scale = 1.0f / sqrtf(static_cast<float>(head_size));
-    const dim3 grid(static_cast<unsigned>(n_tokens) * n_heads);
-    if (type == LPP_F32)
-        hipLaunchKernelGGL((prompt_kernel<float>), grid, dim3(dev::kWave), 0, stream(), static_cast<float*>(d_out), static_cast<const float*>(d_q),
-                           reinterpret_cast<const dev::half_t*>(d_k), reinterpret_cast<const dev::half_t*>(d_v), d_offsets, n_seqs, n_heads,
-                           n_heads / n_kv_heads, head_size, q_stride, kv_stride, out_stride, scale);
-    else
-        hipLaunchKernelGGL((prompt_kernel<dev::half_t>), grid, dim3(dev::kWave), 0, stream(), static_cast<dev::half_t*>(d_out),
-                           static_cast<const dev::half_t*>(d_q), reinterpret_cast<const dev::half_t*>(d_k), reinterpret_cast<const dev::half_t*>(d_v),
-                           d_offsets, n_seqs, n_heads, n_heads / n_kv_heads, head_size, q_stride, kv_stride, out_stride, scale);
-    LPP_CHECK_LAUNCH("prompt_kernel");
-    return LPP_OK;
+    PromptJob job;
+    job.out = d_out;
+    job.q = d_q;
+    job.k = reinterpret_cast<const dev::half_t*>(d_k);
+    job.v = reinterpret_cast<const dev::half_t*>(d_v);
+    job.offsets = d_offsets;
+    job.n_seqs = n_seqs;
+    job.n_tokens = n_tokens;
+    job.shared = n_heads / n_kv_heads;
+    job.n_kv_heads = n_kv_heads;
+    job.q_stride = q_stride;
+    job.kv_stride = kv_stride;
+    job.out_stride = out_stride;
+    if (type == LPP_F32) return head_size == 64 ? launch<float, 64>(job, n_seqs) : launch<float, 128>(job, n_seqs);
+    return head_size == 64 ? launch<dev::half_t, 64>(job, n_seqs) : launch<dev::half_t, 128>(job, n_seqs);
 }
 
 }  // extern "C"
