@@ -59,21 +59,31 @@ inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t 
 
 namespace dev {
 
-// The eight binary16 numbers that a word of codes stands for.  A code in the last bits of a half whose exponent is that of
-// 1024 is 1024 + code, so a pair costs one and-or, one (exact) subtraction and one fused multiply-add, the one rounding.
-__device__ __forceinline__ half8_t kv4_values(uint32_t codes, uint32_t scale_and_low) {
-    const half2_t both = __builtin_bit_cast(half2_t, scale_and_low);
-    const half2_t scale = {both[0], both[0]}, low = {both[1], both[1]}, base = {static_cast<half_t>(1024.0f), static_cast<half_t>(1024.0f)};
-    half8_t v;
+// The eight binary16 numbers that a word of codes stands for.  A code in the last bits of a half whose exponent is that of 1024 is
+// 1024 + code, four bits further up and with the exponent of 64 it is 64 + code: a pair costs one and-or, one (exact) subtraction and one
+// fused multiply-add, the one rounding, and a word one shift.
+struct Kv4Reader {
+    // (in vector registers: v_and_or_b32 takes one constant from a scalar register, the other would make it two instructions)
+    uint32_t as1024 = 0x64006400u, as64 = 0x54005400u;
+    __device__ __forceinline__ Kv4Reader() { asm("" : "+v"(as1024), "+v"(as64)); }
+    __device__ __forceinline__ half8_t operator()(uint32_t codes, uint32_t scale_and_low) const {
+        const half2_t both = __builtin_bit_cast(half2_t, scale_and_low);
+        const half2_t scale = {both[0], both[0]}, low = {both[1], both[1]};
+        const half_t k1024 = static_cast<half_t>(1024.0f), k64 = static_cast<half_t>(64.0f);
+        const uint32_t upper = codes >> 8;
+        half8_t v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = ((codes >> (4 * i)) & 0x000F000Fu) | 0x64006400u;
-        const half2_t pair = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, bits) - base, scale, low);
-        v[2 * i] = pair[0];
-        v[2 * i + 1] = pair[1];
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t from = i < 2 ? codes : upper;
+            const uint32_t bits = (i & 1) ? (from & 0x00F000F0u) | as64 : (from & 0x000F000Fu) | as1024;
+            const half2_t base = (i & 1) ? half2_t{k64, k64} : half2_t{k1024, k1024};
+            const half2_t pair = __builtin_elementwise_fma(__builtin_bit_cast(half2_t, bits) - base, scale, low);
+            v[2 * i] = pair[0];
+            v[2 * i + 1] = pair[1];
+        }
+        return v;
     }
-    return v;
-}
+};
 
 // The sequence that has packed row `row`: the number of sequences that end at or before it (n_seqs: none has it).  `ends`
 // does not decrease.  All lanes of the wavefront call it with the same row and look at 64 ends at a time.

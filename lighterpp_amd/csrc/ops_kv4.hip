@@ -107,12 +107,13 @@ __global__ __launch_bounds__(kLoadThreads) void load_kernel(half_t* __restrict__
     const size_t words = static_cast<size_t>(count) * per_head;
     const size_t i = static_cast<size_t>(blockIdx.x) * kLoadThreads + threadIdx.x;
     if (i >= words) return;
+    const Kv4Reader read;
     half_t* to = blockIdx.z ? v : k;
     const uint32_t* codes = from.codes[blockIdx.z];
     const uint32_t* scales = from.scales[blockIdx.z];
     for (int plane = blockIdx.y; plane < planes; plane += gridDim.y) {
         const size_t at = (static_cast<size_t>(plane) * seq_len + first) * per_head + i;
-        const half8_t values = kv4_values(codes[at], scales[at / 4]);
+        const half8_t values = read(codes[at], scales[at / 4]);
         *reinterpret_cast<half8_t*>(to + (static_cast<size_t>(plane) * words + i) * 8) = values;
     }
 }

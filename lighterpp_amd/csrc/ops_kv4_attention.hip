@@ -13,7 +13,6 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 16;       // of a tile: (16 / shared) new rows x the query heads of a KV head
 constexpr int kStep = 32;       // positions a wavefront takes at a time
-constexpr int kWaves = 4, kThreads = kWave * kWaves;
 constexpr int kMaxSplits = 64;  // ranges that a sequence's positions are cut into
 constexpr float kSlack = 6.0f;
 
@@ -26,17 +25,17 @@ struct AttendJob {
     float2* stats;     // [sequence][KV head][tile][range][16]: maximum (in powers of two) and sum of a range
     float* partials;   // [sequence][KV head][tile][range][16][head_size]
     int n_q, n_kv_heads, shared, seq_len, splits, least, tiles;
+    unsigned per_shared;  // 65536 / shared, rounded up: column * per_shared >> 16 is column / shared for columns below 16
+    // (a start outside -n_q .. seq_len says no more than the ends of that)
+    __device__ __forceinline__ int start_of(int s) const { return min(max(starts[s], -n_q), seq_len); }
+    __device__ __forceinline__ int end_of(int start, int row) const { return min(max(start + row + 1, 0), seq_len); }
+    __device__ __forceinline__ int tokens() const { return static_cast<int>(kRows * per_shared >> 16); }  // of a tile
+    // How many of `positions` a range has: whole steps of four wavefronts, `least` at least.
+    __device__ __forceinline__ int range_of(int positions) const {
+        const int even = (positions + splits - 1) / splits;
+        return max(least, (even + 4 * kStep - 1) / (4 * kStep) * (4 * kStep));
+    }
 };
-
-__device__ __forceinline__ int rows_end(int start, int row, int seq_len) {
-    return static_cast<int>(min(max(static_cast<long long>(start) + row + 1, 0ll), static_cast<long long>(seq_len)));
-}
-// How many positions a range has: whole steps of a workgroup, `least` at least.
-__device__ __forceinline__ int range_of(int positions, int splits, int least) {
-    constexpr int kWhole = kStep * kWaves;
-    const int even = (positions + splits - 1) / splits;
-    return max(least, (even + kWhole - 1) / kWhole * kWhole);
-}
 
 __device__ __forceinline__ float rows_max(float v) {
     const unsigned u = __float_as_uint(v);
@@ -50,8 +49,10 @@ template <int kHs>
 struct Piece {
     static constexpr int kWords = kHs / 32;
     uint32_t codes[kWords], pair;
+    // (a head's rows are within 2^31 bytes: a uniform base and an offset of 32 bits)
     __device__ __forceinline__ void load(const uint32_t* codes_of_head, const uint32_t* scales_of_head, int pos, int part) {
-        const uint32_t* from = codes_of_head + static_cast<size_t>(pos) * (kHs / 8) + part * kWords;
+        const uint32_t row = static_cast<uint32_t>(pos);
+        const char* from = reinterpret_cast<const char*>(codes_of_head) + (row * (kHs / 2) + static_cast<uint32_t>(part) * (kWords * 4));
         if constexpr (kWords == 4) {
             const uintx4 all = load16(from);
 #pragma unroll
@@ -61,9 +62,10 @@ struct Piece {
             codes[0] = all.x;
             codes[1] = all.y;
         }
-        pair = scales_of_head[static_cast<size_t>(pos) * (kHs / kKv4Group) + part * kWords / 4];
+        pair = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(scales_of_head) +
+                                                  (row * (kHs / 8) + static_cast<uint32_t>(part * kWords / 4) * 4));
     }
-    __device__ __forceinline__ half8_t values(int i) const { return kv4_values(codes[i], pair); }
+    __device__ __forceinline__ half8_t values(const Kv4Reader& read, int i) const { return read(codes[i], pair); }
     // Whether a value may be infinite or NaN.
     __device__ __forceinline__ bool may_be_nonfinite() const {
         const half2_t both = __builtin_bit_cast(half2_t, pair);
@@ -71,46 +73,76 @@ struct Piece {
     }
 };
 
-// Q of a tile as B operands: column lane % 16, the values that a K piece's words have; heads and remainders.
+// Q of a tile as B operands: column lane % 16, the values that a K piece's words have; heads and remainders.  Heads of 128 have them in LDS, the
+// same for all wavefronts of a workgroup: in registers they are 32 of them, and with 168 for three wavefronts to a SIMD the loop spills, whose
+// reloads wait for the K and V rows that are on their way.
 template <int kHs>
 struct Queries {
     static constexpr int kWords = kHs / 32;
-    half8_t high[kWords], low[kWords];
-    __device__ __forceinline__ void load(const float* row, int part) {
+    static constexpr bool kInLds = kHs == 128;
+    static constexpr int kLdsBytes = kInLds ? 2 * kWords * 16 * kWave : 0;
+    half8_t held[kInLds ? 1 : 2 * kWords];  // [word][head, remainder]
+    const half8_t* shared;
+    // wave, waves: this wavefront's share of the work (a barrier has to follow)
+    __device__ __forceinline__ void load(const float* row, int part, char* lds, int wave, int waves) {
+        half8_t* to = reinterpret_cast<half8_t*>(lds) + lane_id();
+        shared = to;
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
+            if (kInLds && i % waves != wave) continue;
             const float* from = row + part * kWords * 8 + 8 * i;
             const floatx4 a = as_float4(load16(from)), b = as_float4(load16(from + 4));
+            half8_t high, low;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float v = e < 4 ? a[e & 3] : b[e & 3];
-                high[i][e] = static_cast<half_t>(v);
-                low[i][e] = static_cast<half_t>(v - static_cast<float>(high[i][e]));
+                high[e] = static_cast<half_t>(v);
+                low[e] = static_cast<half_t>(v - static_cast<float>(high[e]));
+            }
+            if constexpr (kInLds) {
+                to[2 * i * kWave] = high;
+                to[(2 * i + 1) * kWave] = low;
+            } else {
+                held[2 * i] = high;
+                held[2 * i + 1] = low;
             }
         }
     }
-    // scores of 16 positions: lane: column lane % 16, positions 4 (lane / 16) ..
-    __device__ __forceinline__ floatx4 scores(const Piece<kHs>& k) const {
-        floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    // scores of n x 16 positions: lane: column lane % 16, positions 4 (lane / 16) ..
+    template <int n>
+    __device__ __forceinline__ void scores(const Kv4Reader& read, const Piece<kHs>* k, floatx4* st) const {
+#pragma unroll
+        for (int t = 0; t < n; ++t) st[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
-            const half8_t kv = k.values(i);
-            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, high[i], s, 0, 0, 0);
-            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, low[i], s, 0, 0, 0);
+            half8_t high, low;
+            if constexpr (kInLds) {
+                high = shared[2 * i * kWave];
+                low = shared[(2 * i + 1) * kWave];
+            } else {
+                high = held[2 * i];
+                low = held[2 * i + 1];
+            }
+#pragma unroll
+            for (int t = 0; t < n; ++t) {
+                const half8_t kv = k[t].values(read, i);
+                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, high, st[t], 0, 0, 0);
+                st[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, low, st[t], 0, 0, 0);
+            }
         }
-        return s;
     }
 };
 
 // Which row a column of a tile is.
 struct Column {
-    int token, head;
+    int in_tile, token, head;
     bool valid;
     __device__ __forceinline__ Column(const AttendJob& job, int tile, int column) {
-        const int tokens = kRows / job.shared;
-        token = tile * tokens + column / job.shared;
-        head = column % job.shared;
-        valid = column < tokens * job.shared && token < job.n_q;
+        const int tokens = job.tokens();
+        in_tile = static_cast<int>(column * job.per_shared >> 16);
+        head = column - in_tile * job.shared;
+        token = tile * tokens + in_tile;
+        valid = in_tile < tokens && token < job.n_q;
         token = min(token, min(tile * tokens + tokens, job.n_q) - 1);
     }
     __device__ __forceinline__ size_t at(const AttendJob& job, int s, int kvh) const {
@@ -118,25 +150,25 @@ struct Column {
     }
 };
 
-template <int kHs>
-__global__ __launch_bounds__(kThreads) void attend_kernel(AttendJob job) {
-    constexpr int kDTiles = kHs / 16, kWords = kHs / 32, kRowBytes = 2 * kHs;
+template <int kHs, int kWaves>
+__global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kernel(AttendJob job) {
+    constexpr int kDTiles = kHs / 16, kWords = kHs / 32, kRowBytes = 2 * kHs, kThreads = kWave * kWaves;
     constexpr int kPad = kHs + 4, kPart = kRows * kPad + 2 * kRows;  // floats a wavefront leaves for the merge
     constexpr int kWaveBytes = kPart * 4;
     static_assert(kWaveBytes >= kStep * kRowBytes, "V rows of a step");
-    __shared__ __align__(16) char lds[kWaves * kWaveBytes];
+    extern __shared__ __align__(16) char lds[];
     const int lane = lane_id(), wave = wave_index(), column = lane & 15, part = lane >> 4;
     const int split = static_cast<int>(blockIdx.x) % job.splits, tile = static_cast<int>(blockIdx.x) / job.splits, kvh = blockIdx.y, s = blockIdx.z;
-    const int tokens = kRows / job.shared, start = job.starts[s];
-    const int all_end = rows_end(start, job.n_q - 1, job.seq_len);
-    const int range = range_of(all_end, job.splits, job.least);
+    const int tokens = job.tokens(), start = job.start_of(s);
+    const int all_end = job.end_of(start, job.n_q - 1);
+    const int range = job.range_of(all_end);
     const int begin = split * range;
     if (begin >= all_end && split > 0) return;
-    const int tile_end = rows_end(start, min(tile * tokens + tokens, job.n_q) - 1, job.seq_len);
+    const int tile_end = job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1);
     const int end = min(begin + range, tile_end);  // (at or before `begin`: the tile's rows attend to nothing here)
     const bool only = range >= all_end;            // (uniform over the sequence: no merge)
     const Column mine(job, tile, column);
-    const int my_end = rows_end(start, mine.token, job.seq_len), first_end = rows_end(start, tile * tokens, job.seq_len);
+    const int my_end = job.end_of(start, mine.token), first_end = job.end_of(start, tile * tokens);
     const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
     const uint32_t* codes[2];
     const uint32_t* scales[2];
@@ -145,8 +177,21 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendJob job) {
         codes[w] = job.cache.codes[w] + head_rows * (kHs / 8);
         scales[w] = job.cache.scales[w] + head_rows * (kHs / kKv4Group);
     }
+    // K and V of a step travel while the step before is worked on, each requested as soon as its registers are free.
+    Piece<kHs> k[2], v[2];
+    auto request = [&](Piece<kHs>(&to)[2], int which, int p0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) to[t].load(codes[which], scales[which], min(p0 + 16 * t + column, end - 1), part);
+    };
+    const int first = begin + wave * kStep;
+    if (first < end) {
+        request(k, 0, first);
+        request(v, 1, first);
+    }
     Queries<kHs> q;
-    q.load(job.q + mine.at(job, s, kvh) * kHs, part);
+    q.load(job.q + mine.at(job, s, kvh) * kHs, part, lds + kWaves * kWaveBytes, wave, kWaves);
+    if constexpr (Queries<kHs>::kInLds) __syncthreads();
+    const Kv4Reader read;
 
     floatx4 o[kDTiles];
 #pragma unroll
@@ -161,48 +206,33 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendJob job) {
     // conflicts
     char* values = lds + wave * kWaveBytes;
     auto swizzle = [](int row) { return kHs == 64 ? 2 * ((row >> 1) & 3) : 4 * (row & 3) + ((row >> 2) & 3); };
-    int v_at[kDTiles];
+    int v_at[kDTiles], v_to[kWords];  // (of the first sixteen positions; the others are 16 rows further, in the same order)
     {
         const int row = 4 * part + ((lane & 15) >> 2);
 #pragma unroll
         for (int dt = 0; dt < kDTiles; ++dt) v_at[dt] = row * kRowBytes + 16 * ((2 * dt + ((lane & 3) >> 1)) ^ swizzle(row)) + 8 * (lane & 1);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) v_to[i] = column * kRowBytes + 16 * ((kWords * part + i) ^ swizzle(column));
     }
 
-    Piece<kHs> next[2][2];  // [K, V][first, second sixteen positions]
-    auto request = [&](int p0) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int w = 0; w < 2; ++w) next[w][t].load(codes[w], scales[w], min(p0 + 16 * t + column, end - 1), part);
-    };
-    const int first = begin + wave * kStep;
-    if (first < end) request(first);
     for (int p0 = first; p0 < end; p0 += kStep * kWaves) {
-        Piece<kHs> now[2][2];
+        const bool more = p0 + kStep * kWaves < end;  // (uniform)
+        const bool partly = p0 + kStep > first_end;   // (uniform) some row does not attend to the whole step
+        floatx4 st[2];
+        q.template scores<2>(read, k, st);
+        if (more) request(k, 0, p0 + kStep * kWaves);
+        // V rows behind the tile's last position are zero: a weight of zero does not keep an infinity or NaN out.
+        if (partly) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (p0 + 16 * t + column >= tile_end) v[t].pair = 0u;
+        }
+        const bool odd = __builtin_amdgcn_ballot_w64(v[0].may_be_nonfinite() || v[1].may_be_nonfinite()) != 0ull;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int w = 0; w < 2; ++w) now[w][t] = next[w][t];
-        if (p0 + kStep * kWaves < end) request(p0 + kStep * kWaves);
-        const bool partly = p0 + kStep > first_end;  // (uniform) some row does not attend to the whole step
-        floatx4 st[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) st[t] = q.scores(now[0][t]);
-        // V into LDS.  Rows behind the tile's last position are cleared: a weight of zero does not keep an infinity or NaN out.
-        bool odd = false;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int row = 16 * t + column;
-            const bool live = p0 + row < tile_end;
-            odd = odd || (live && now[1][t].may_be_nonfinite());
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                half8_t v = now[1][t].values(i);
-                if (partly && !live) v = half8_t{};
-                *reinterpret_cast<half8_t*>(values + row * kRowBytes + 16 * ((kWords * part + i) ^ swizzle(row))) = v;
-            }
-        }
-        odd = __builtin_amdgcn_ballot_w64(odd) != 0ull;
+            for (int i = 0; i < kWords; ++i) *reinterpret_cast<half8_t*>(values + v_to[i] + 16 * t * kRowBytes) = v[t].values(read, i);
+        if (more) request(v, 1, p0 + kStep * kWaves);
         if (partly) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -226,7 +256,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendJob job) {
             seen = seen || moves;
         }
         half8_t ph, pl;
-        float step_sum = 0.0f;
+        float step_sum = 0.0f;  // (of its own, so that the running sum is rounded once a step)
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
             const float p_0 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], scale, -top)), p_1 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][(e & 3) + 1], scale, -top));
@@ -241,8 +271,7 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendJob job) {
             pl[e + 1] = static_cast<half_t>(fmaf(static_cast<float>(h[1]), minus_one, p_1));
         }
         lsum += step_sum;
-#pragma unroll
-        for (int dt = 0; dt < kDTiles; ++dt) {
+        auto values_of = [&](int dt) {
             union {
                 short4_t half[2];
                 half8_t whole;
@@ -250,207 +279,254 @@ __global__ __launch_bounds__(kThreads) void attend_kernel(AttendJob job) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
                 vf.half[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(values + v_at[dt] + 16 * t * kRowBytes));
-            if (odd) {
-                // (uniform) An infinity or NaN, perhaps, among the step's V rows: one token after the other, with the rows behind it cleared; a
-                // lane's output is its own token's.  The weights' remainders, of either sign, meet the finite values only.
+            return vf.whole;
+        };
+        if (odd) {
+            // (uniform) An infinity or NaN, perhaps, among the step's V rows: one token after the other, with the rows behind it cleared; a
+            // lane's output is its own token's.  The weights' remainders, of either sign, meet the finite values only.
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt) {
+                const half8_t all = values_of(dt);
                 for (int token = 0; token < tokens; ++token) {
-                    const int token_end = rows_end(start, tile * tokens + token, job.seq_len) - p0 - 4 * part;
-                    half8_t v = vf.whole;
+                    const int token_end = job.end_of(start, tile * tokens + token) - p0 - 4 * part;
+                    half8_t x = all;
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if ((e & 3) + 16 * (e >> 2) >= token_end) v[e] = static_cast<half_t>(0.0f);
-                    floatx4 with = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[dt], 0, 0, 0);
+                        if ((e & 3) + 16 * (e >> 2) >= token_end) x[e] = static_cast<half_t>(0.0f);
+                    floatx4 with = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph, o[dt], 0, 0, 0);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (!(fabsf(static_cast<float>(v[e])) < INFINITY)) v[e] = static_cast<half_t>(0.0f);
-                    with = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, with, 0, 0, 0);
-                    if (column / job.shared == token) o[dt] = with;
+                        if (!(fabsf(static_cast<float>(x[e])) < INFINITY)) x[e] = static_cast<half_t>(0.0f);
+                    with = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl, with, 0, 0, 0);
+                    if (mine.in_tile == token) o[dt] = with;
                 }
-            } else {
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.whole, ph, o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf.whole, pl, o[dt], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < kDTiles; ++dt) {
+                const half8_t x = values_of(dt);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ph, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, pl, o[dt], 0, 0, 0);
             }
         }
     }
     lsum = rows_sum(lsum);
     if (!seen) top = -INFINITY;
 
-    // The wavefronts meet in LDS, each thread adding four values of a row in the order of the wavefronts.
+    // The wavefronts meet in LDS, each thread adding four values of a row in the order of the wavefronts.  Those that had no step have left
+    // nothing and are not read.
+    const int steps = max((end - begin + kStep - 1) / kStep, 0), parts = max(min(steps, kWaves), 1);
     float* all = reinterpret_cast<float*>(lds);
-    float* my_part = all + wave * kPart;
-    // (its own V rows are read: the values are in registers)
+    if (wave < parts) {
+        float* my_part = all + wave * kPart;
 #pragma unroll
-    for (int dt = 0; dt < kDTiles; ++dt) *reinterpret_cast<floatx4*>(my_part + column * kPad + 16 * dt + 4 * part) = o[dt];
-    if (part == 0) {
-        my_part[kRows * kPad + column] = top;
-        my_part[kRows * kPad + kRows + column] = lsum;
+        for (int dt = 0; dt < kDTiles; ++dt) *reinterpret_cast<floatx4*>(my_part + column * kPad + 16 * dt + 4 * part) = o[dt];
+        if (part == 0) {
+            my_part[kRows * kPad + column] = top;
+            my_part[kRows * kPad + kRows + column] = lsum;
+        }
     }
     __syncthreads();
     const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits + split;
     constexpr int kFours = kHs / 4;
-    for (int i = threadIdx.x; i < kRows * kFours; i += kThreads) {
+    const int used = min(tokens, job.n_q - tile * tokens) * job.shared;  // rows there are
+    for (int i = threadIdx.x; i < used * kFours; i += kThreads) {
         const int row = i / kFours, four = i % kFours;
-        const Column its(job, tile, row);
-        if (!its.valid) continue;
-        float weight[kWaves], all_top = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            weight[w] = all[w * kPart + kRows * kPad + row];
-            all_top = fmaxf(all_top, weight[w]);
-        }
+        float all_top = -INFINITY, total = 0.0f;
+        for (int w = 0; w < parts; ++w) all_top = fmaxf(all_top, all[w * kPart + kRows * kPad + row]);
         const float reference = all_top == -INFINITY ? 0.0f : all_top;  // (nothing seen, or no score was a number)
-        floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            weight[w] = __builtin_amdgcn_exp2f(weight[w] - reference);
-            total = fmaf(all[w * kPart + kRows * kPad + kRows + row], weight[w], total);
+        floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int w = 0; w < parts; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(all[w * kPart + kRows * kPad + row] - reference);
+            total = fmaf(all[w * kPart + kRows * kPad + kRows + row], weight, total);
             const floatx4 a = *reinterpret_cast<const floatx4*>(all + w * kPart + row * kPad + 4 * four);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = fmaf(a[u], weight[w], v[u]);
+            for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[u], weight, sum[u]);
         }
         if (only) {
-            const bool any = rows_end(start, its.token, job.seq_len) > 0;
+            const Column its(job, tile, row);
+            const bool any = job.end_of(start, its.token) > 0;
             const float inverse = 1.0f / total;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = any ? v[u] * inverse : 0.0f;
-            *reinterpret_cast<floatx4*>(job.out + its.at(job, s, kvh) * kHs + 4 * four) = v;
+            for (int u = 0; u < 4; ++u) sum[u] = any ? sum[u] * inverse : 0.0f;
+            *reinterpret_cast<floatx4*>(job.out + its.at(job, s, kvh) * kHs + 4 * four) = sum;
         } else {
-            *reinterpret_cast<floatx4*>(job.partials + (slot * kRows + row) * kHs + 4 * four) = v;
+            *reinterpret_cast<floatx4*>(job.partials + (slot * kRows + row) * kHs + 4 * four) = sum;
         }
         if (four == 0) job.stats[slot * kRows + row] = make_float2(all_top, total);
     }
 }
 
-// What is left once every range has been walked: blocks before job.tiles (where there are ranges to merge) merge a tile's rows, the others add up
+// What is left once every range has been walked: blocks before `merges` (where there are ranges to merge) merge a row each, the others add up
 // the weights of kMassPositions positions each.
-constexpr int kMassPositions = 2 * kStep * kWaves;
+constexpr int kFinishWaves = 4, kFinishThreads = kWave * kFinishWaves;
+constexpr int kMassPositions = 256;
 
 template <int kHs>
-__global__ __launch_bounds__(kThreads) void finish_kernel(AttendJob job, int merges) {
-    __shared__ float weights[kRows][kMaxSplits];
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges) {
+    constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours;
+    __shared__ float weights[kMaxSplits];
+    __shared__ __align__(16) float partial[kSlices][kHs];
     __shared__ float tops[kRows], inverses[kRows];
+    __shared__ __align__(16) char q_lds[Queries<kHs>::kLdsBytes > 0 ? Queries<kHs>::kLdsBytes : 16];
     const int lane = lane_id(), wave = wave_index(), column = lane & 15, part = lane >> 4;
-    const int kvh = blockIdx.y, s = blockIdx.z, start = job.starts[s], tokens = kRows / job.shared;
-    const int all_end = rows_end(start, job.n_q - 1, job.seq_len);
-    const int range = range_of(all_end, job.splits, job.least), active = max((all_end + range - 1) / range, 1);
-    const bool merging = static_cast<int>(blockIdx.x) < merges;
-    if (merging && active == 1) return;
-    const int p_first = (static_cast<int>(blockIdx.x) - merges) * kMassPositions;
-    if (!merging && p_first >= all_end) return;
-
-    // (maximum, 1 / sum) of a tile's rows, and every range's weight in them; 16 threads to a row
-    auto combine = [&](int tile) {
+    const int kvh = blockIdx.y, s = blockIdx.z, start = job.start_of(s), tokens = job.tokens();
+    const int all_end = job.end_of(start, job.n_q - 1);
+    const int range = job.range_of(all_end), active = max((all_end + range - 1) / range, 1);
+    if (static_cast<int>(blockIdx.x) < merges) {
+        if (active == 1) return;
+        const int tile = static_cast<int>(blockIdx.x) / kRows, row = static_cast<int>(blockIdx.x) % kRows;
+        const Column its(job, tile, row);
+        if (!its.valid) return;
         const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
-        const int row = threadIdx.x / 16, at = threadIdx.x % 16;
-        const bool live = Column(job, tile, row).valid;
-        float2 st[kMaxSplits / 16];
-        float top = -INFINITY, total = 0.0f;
+        // (the ranges' outputs are requested along with their weights; a range that the row does not attend to has left none)
+        const int slice = static_cast<int>(threadIdx.x) / kFours, four = static_cast<int>(threadIdx.x) % kFours;
+        constexpr int kEach = kMaxSplits / kSlices;
+        floatx4 a[kEach];
 #pragma unroll
-        for (int i = 0; i < kMaxSplits / 16; ++i) {
-            st[i] = live && at + 16 * i < active ? job.stats[(slot + at + 16 * i) * kRows + row] : make_float2(-INFINITY, 0.0f);
-            top = fmaxf(top, st[i].x);
+        for (int i = 0; i < kEach; ++i) {
+            const int at = min(slice + kSlices * i, active - 1);
+            a[i] = *reinterpret_cast<const floatx4*>(job.partials + ((slot + at) * kRows + row) * kHs + 4 * four);
         }
-        top = fmaxf(top, dpp_move<kDppXor1>(top));
-        top = fmaxf(top, dpp_move<kDppXor2>(top));
-        top = fmaxf(top, dpp_move<kDppHalfMirror>(top));
-        top = fmaxf(top, dpp_move<kDppMirror>(top));
+        const float2 st = lane < active ? job.stats[(slot + lane) * kRows + row] : make_float2(-INFINITY, 0.0f);
+        float top = wave_max(st.x);
         if (top == -INFINITY) top = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kMaxSplits / 16; ++i) {
-            const float w = __builtin_amdgcn_exp2f(st[i].x - top);
-            // (a range that the row does not attend to has left no output)
-            weights[row][at + 16 * i] = st[i].x == -INFINITY && st[i].y == 0.0f ? -1.0f : w;
-            total = fmaf(st[i].y, w, total);
-        }
-        total = row16_sum(total);
-        if (at == 0) {
-            tops[row] = top;
-            inverses[row] = live ? 1.0f / total : 0.0f;
-        }
-    };
-    if (merging) {
-        const int tile = blockIdx.x;
-        combine(tile);
+        const float weight = __builtin_amdgcn_exp2f(st.x - top);
+        const float total = wave_sum(st.y * weight);
+        if (wave == 0) weights[lane] = st.x == -INFINITY && st.y == 0.0f ? -1.0f : weight;
         __syncthreads();
-        const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
-        constexpr int kFours = kHs / 4;
-        for (int i = threadIdx.x; i < kRows * kFours; i += kThreads) {
-            const int row = i / kFours, four = i % kFours;
-            const Column its(job, tile, row);
-            if (!its.valid) continue;
-            floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            const float* from = job.partials + (slot * kRows + row) * kHs + 4 * four;
-#pragma unroll 8
-            for (int k = 0; k < active; ++k) {
-                const float w = weights[row][k];
-                if (w < 0.0f) continue;
-                const floatx4 a = *reinterpret_cast<const floatx4*>(from + static_cast<size_t>(k) * kRows * kHs);
+        floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = fmaf(a[u], w, v[u]);
-            }
-            const bool any = rows_end(start, its.token, job.seq_len) > 0;
+        for (int i = 0; i < kEach; ++i) {
+            const int at = slice + kSlices * i;
+            const float w = weights[at];
+            if (at < active && w >= 0.0f)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = any ? v[u] * inverses[row] : 0.0f;
-            *reinterpret_cast<floatx4*>(job.out + its.at(job, s, kvh) * kHs + 4 * four) = v;
+                for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[i][u], w, sum[u]);
+        }
+        *reinterpret_cast<floatx4*>(&partial[slice][4 * four]) = sum;
+        __syncthreads();
+        if (threadIdx.x < kHs) {
+            float v = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) v += partial[i][threadIdx.x];
+            job.out[its.at(job, s, kvh) * kHs + threadIdx.x] = job.end_of(start, its.token) > 0 ? v / total : 0.0f;
         }
         return;
     }
+    const int p_first = (static_cast<int>(blockIdx.x) - merges) * kMassPositions;
+    if (p_first >= all_end) return;
     const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
     const uint32_t* codes = job.cache.codes[0] + head_rows * (kHs / 8);
     const uint32_t* scales = job.cache.scales[0] + head_rows * (kHs / kKv4Group);
+    float* mass = job.mass + head_rows;
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
-    constexpr int kPieces = kMassPositions / (kWaves * 16);
+    constexpr int kPieces = kMassPositions / (16 * kFinishWaves);
     Piece<kHs> k[kPieces];
-    floatx4 sum[kPieces];
+    floatx4 sum[kPieces];  // of this lane's column, over the tiles
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-        k[i].load(codes, scales, min(p_first + 16 * (wave + kWaves * i) + column, all_end - 1), part);
+        k[i].load(codes, scales, min(p_first + 16 * (wave + kFinishWaves * i) + column, all_end - 1), part);
         sum[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    // (a lane adds the weights of one position a piece: position 4 part + column, for columns below four)
+    float before[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int p = p_first + 16 * (wave + kFinishWaves * i) + 4 * part + column;
+        before[i] = column < 4 && p < all_end ? mass[p] : 0.0f;
+    }
+    const Kv4Reader read;
     for (int tile = 0; tile < job.tiles; ++tile) {
-        if (rows_end(start, min(tile * tokens + tokens, job.n_q) - 1, job.seq_len) <= p_first) continue;  // (uniform)
+        if (job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1) <= p_first) continue;  // (uniform)
         const Column mine(job, tile, column);
-        const int my_end = rows_end(start, mine.token, job.seq_len);
+        const int my_end = mine.valid ? job.end_of(start, mine.token) : 0;
+        if (tile > 0) __syncthreads();  // (the tile before is done with what LDS holds)
         Queries<kHs> q;
-        q.load(job.q + mine.at(job, s, kvh) * kHs, part);
-        __syncthreads();
-        combine(tile);
+        q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds, wave, kFinishWaves);
+        // (maximum, 1 / sum) of the tile's rows: 16 threads to a row
+        {
+            const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
+            const int row = threadIdx.x / 16, at = threadIdx.x % 16;
+            const bool live = row < min(tokens, job.n_q - tile * tokens) * job.shared;
+            float2 st[kMaxSplits / 16];
+            float top = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kMaxSplits / 16; ++i) {
+                st[i] = make_float2(-INFINITY, 0.0f);
+                if (live && at + 16 * i < active) st[i] = job.stats[(slot + at + 16 * i) * kRows + row];
+                top = fmaxf(top, st[i].x);
+            }
+            top = fmaxf(top, dpp_move<kDppXor1>(top));
+            top = fmaxf(top, dpp_move<kDppXor2>(top));
+            top = fmaxf(top, dpp_move<kDppHalfMirror>(top));
+            top = fmaxf(top, dpp_move<kDppMirror>(top));
+            if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kMaxSplits / 16; ++i) total = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - top), total);
+            total = row16_sum(total);
+            if (at == 0) {
+                tops[row] = top;
+                inverses[row] = 1.0f / total;
+            }
+        }
         __syncthreads();
         const float top = tops[column], inverse = inverses[column];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int p0 = p_first + 16 * (wave + kWaves * i) + 4 * part;
-            const floatx4 st = q.scores(k[i]);
+        for (int i = 0; i < kPieces; i += 2) {
+            floatx4 st[2];
+            q.template scores<2>(read, k + i, st);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(st[e], scale, -top)) * inverse;
-                sum[i][e] += row16_sum(mine.valid && p0 + e < my_end ? w : 0.0f);
-            }
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -top)) * inverse;
+                    sum[i + t][e] += p_first + 16 * (wave + kFinishWaves * (i + t)) + 4 * part + e < my_end ? w : 0.0f;
+                }
         }
     }
-    float* mass = job.mass + head_rows;
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
-        const int p0 = p_first + 16 * (wave + kWaves * i) + 4 * part;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (column == e && p0 + e < all_end) mass[p0 + e] += sum[i][e];
+        for (int e = 0; e < 4; ++e) sum[i][e] = row16_sum(sum[i][e]);
+        const int p = p_first + 16 * (wave + kFinishWaves * i) + 4 * part + column;
+        if (column < 4 && p < all_end) mass[p] = before[i] + (column == 0 ? sum[i][0] : column == 1 ? sum[i][1] : column == 2 ? sum[i][2] : sum[i][3]);
     }
 }
 
 int tiles_of(int n_q, int shared) { return (n_q + kRows / shared - 1) / (kRows / shared); }
 
-// Ranges a sequence's positions are cut into, and the least positions of one.
+// Ranges a sequence's positions are cut into, the least positions of one, and the wavefronts to one.
 struct Split {
-    int splits, least;
+    int splits, least, waves;
 };
 Split split_of(const lpp_kv4_shape& shape, int tiles) {
     const long long heads = static_cast<long long>(shape.n_seqs) * shape.n_kv_heads * tiles;
     Split s;
-    s.least = heads >= 2ll * compute_units() ? 1024 : heads * 4 >= compute_units() ? 512 : 256;
+    s.waves = heads * 4 > compute_units() ? 4 : shape.head_size == 64 ? 16 : 8;
+    s.least = heads >= 2ll * compute_units() ? 2048 : heads * 4 > compute_units() ? 1024 : 512;
     const int most = (shape.seq_len + s.least - 1) / s.least;
     s.splits = most < kMaxSplits ? most : kMaxSplits;
     return s;
+}
+
+template <int kHs, int kWaves>
+lpp_status launch_attend(const AttendJob& job, dim3 grid) {
+    constexpr int kLds = kWaves * (kRows * (kHs + 4) + 2 * kRows) * 4 + Queries<kHs>::kLdsBytes;
+    const auto kernel = &attend_kernel<kHs, kWaves>;
+    if constexpr (kLds > 64 * 1024) {  // told to the runtime once per device
+        static bool sized[64] = {};
+        int device = 0;
+        LPP_HIP(hipGetDevice(&device));
+        if (device < 0 || device >= 64 || !sized[device]) {
+            LPP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+            if (device >= 0 && device < 64) sized[device] = true;
+        }
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(kWave * kWaves), kLds, stream(), job);
+    LPP_CHECK_LAUNCH("attend_kernel");
+    return LPP_OK;
 }
 
 lpp_status check(const char* who, const lpp_kv4_shape* shape, int n_heads, int n_q) {
@@ -507,23 +583,23 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     const Split split = split_of(*shape, job.tiles);
     job.splits = split.splits;
     job.least = split.least;
+    job.per_shared = (65536u + job.shared - 1) / job.shared;
     const size_t slots = static_cast<size_t>(shape->n_seqs) * shape->n_kv_heads * job.tiles * job.splits;
     job.stats = static_cast<float2*>(d_workspace);
     job.partials = reinterpret_cast<float*>(job.stats + slots * kRows);
     const dim3 grid(static_cast<unsigned>(job.splits) * job.tiles, shape->n_kv_heads, shape->n_seqs);
     if (shape->head_size == 64)
-        hipLaunchKernelGGL(attend_kernel<64>, grid, dim3(kThreads), 0, stream(), job);
+        LPP_TRY(split.waves == 16 ? (launch_attend<64, 16>(job, grid)) : (launch_attend<64, 4>(job, grid)));
     else
-        hipLaunchKernelGGL(attend_kernel<128>, grid, dim3(kThreads), 0, stream(), job);
-    LPP_CHECK_LAUNCH("attend_kernel");
-    const int merges = job.splits > 1 ? job.tiles : 0;
+        LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
+    const int merges = job.splits > 1 ? job.tiles * kRows : 0;
     const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + kMassPositions - 1) / kMassPositions : 0);
     if (blocks > 0) {
         const dim3 rest(blocks, shape->n_kv_heads, shape->n_seqs);
         if (shape->head_size == 64)
-            hipLaunchKernelGGL(finish_kernel<64>, rest, dim3(kThreads), 0, stream(), job, merges);
+            hipLaunchKernelGGL(finish_kernel<64>, rest, dim3(kFinishThreads), 0, stream(), job, merges);
         else
-            hipLaunchKernelGGL(finish_kernel<128>, rest, dim3(kThreads), 0, stream(), job, merges);
+            hipLaunchKernelGGL(finish_kernel<128>, rest, dim3(kFinishThreads), 0, stream(), job, merges);
         LPP_CHECK_LAUNCH("finish_kernel");
     }
     return LPP_OK;
