@@ -23,24 +23,66 @@ __device__ __forceinline__ int quad_or(int v) {
     return v | dpp_move_i<kDppXor2>(v);
 }
 
-// The integer nearest to (x - low) / scale, in 0 .. 15.  In fp32 the quotient is off by less than 16 * 3 * 2^-24 where the
-// result is not cut, so only a quotient within 1e-5 of a border is formed again, in 64 bits (one value in 50000).
-__device__ __forceinline__ uint32_t code_of(float x, float low, float scale, float inverse) {
-    const float t = (x - low) * inverse;
-    float k = rintf(t);
-    if (fabsf(t - k) > 0.5f - 1e-5f && scale > 0.0f)
-        k = static_cast<float>(rint((static_cast<double>(x) - static_cast<double>(low)) / static_cast<double>(scale)));
-    return static_cast<uint32_t>(fminf(fmaxf(k, 0.0f), 15.0f));
+// A word of the codes of eight values: the integers nearest to (x - low) / scale, in 0 .. 15.  In fp32 the quotient, cut to that range, is off by less
+// than 16 * 5 * 2^-24 (difference, reciprocal, product), so a word with a quotient within 1e-5 of a border, one in 6000, is formed
+// again in 64 bits.  Adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the lowest bits: the codes are added up
+// with what is above them, which is taken off at the end.
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float scale) {
+    const float inverse = scale > 0.0f ? __builtin_amdgcn_rcpf(scale) : 0.0f;
+    uint32_t word = 0, above = 0;
+    float furthest = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float t = __builtin_amdgcn_fmed3f((x[e] - low) * inverse, 0.0f, 15.0f), shifted = t + 8388608.0f;
+        furthest = fmaxf(furthest, fabsf(t - (shifted - 8388608.0f)));
+        word += __float_as_uint(shifted) << (4 * (e / 2) + 16 * (e & 1));
+        above += 0x4B000000u << (4 * (e / 2) + 16 * (e & 1));
+    }
+    word -= above;
+    if (furthest > 0.5f - 1e-5f) {
+        word = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const double t = rint((static_cast<double>(x[e]) - static_cast<double>(low)) / static_cast<double>(scale));
+            word |= static_cast<uint32_t>(fmin(fmax(t, 0.0), 15.0)) << (4 * (e / 2) + 16 * (e & 1));
+        }
+    }
+    return word;
 }
 
-// One wavefront per row of K or V; a lane has a word's eight values.
+// r / 15 rounded to nearest: the product with the rounded reciprocal, and once more with what it leaves (equal to the quotient
+// for every mantissa; results that a binary16 rounds to 0 aside).  The result is hidden from the compiler, which would otherwise
+// form the last step and its rounding to binary16 in one instruction, with one rounding.
+__device__ __forceinline__ float fifteenth(float r) {
+    constexpr float kInverse = 1.0f / 15.0f;
+    const float q = r * kInverse;
+    float quotient = fmaf(fmaf(q, -15.0f, r), kInverse, q);
+    asm("" : "+v"(quotient));
+    return quotient;
+}
+
+// One wavefront per row of K or V; a lane has a word's eight values, two words at a time.  The first values are requested before anything is
+// known about the row's sequence.
 template <typename T>
 __global__ __launch_bounds__(kStoreThreads) void store_kernel(Kv4Layer to, const T* __restrict__ k, const T* __restrict__ v, int stride,
                                                               const int* __restrict__ offsets, const int* __restrict__ starts, int n_tokens,
                                                               int n_seqs, int n_kv_heads, int head_size, int seq_len) {
+    constexpr int kAtOnce = 2, kLoads = sizeof(T) / 2;  // words; requests of 16 bytes to a word
     const int wave = wave_index(), lane = lane_id();
     const int row = static_cast<int>(blockIdx.x) * 2 + wave / 2, which = wave & 1;
     if (row >= n_tokens) return;
+    const T* from = (which ? v : k) + static_cast<size_t>(row) * stride;
+    const int words = n_kv_heads * head_size / 8, per_head = head_size / 8;
+    uintx4 raw[kAtOnce][kLoads];
+    auto request = [&](int w0) {
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int w = min(w0 + kWave * u + lane, words - 1);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) raw[u][i] = load16(from + 8 * w + 8 / kLoads * i);
+        }
+    };
+    request(0);
     int s, first;
     if (offsets != nullptr) {
         s = sequence_of_row(offsets + 1, n_seqs, row);
@@ -54,49 +96,48 @@ __global__ __launch_bounds__(kStoreThreads) void store_kernel(Kv4Layer to, const
     }
     const long long pos = (starts != nullptr ? static_cast<long long>(starts[s]) : 0ll) + row - first;
     if (pos < 0 || pos >= seq_len) return;
-    const T* from = (which ? v : k) + static_cast<size_t>(row) * stride;
     uint32_t* codes = to.codes[which];
     uint32_t* scales = to.scales[which];
-    const int words = n_kv_heads * head_size / 8, per_head = head_size / 8;
-    for (int w = lane; w < words; w += kWave) {
-        float x[8];
-        if constexpr (sizeof(T) == 2) {
-            const half8_t h = as_half8(load16(from + 8 * w));
+    const int shift = per_head == 8 ? 3 : 4;
+    const size_t base = static_cast<size_t>(s) * n_kv_heads * seq_len + static_cast<size_t>(pos);
+    for (int w0 = 0; w0 < words; w0 += kAtOnce * kWave) {
+        float x[kAtOnce][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(h[e]);
-        } else {
-            const floatx4 a = as_float4(load16(from + 8 * w)), b = as_float4(load16(from + 8 * w + 4));
+        for (int u = 0; u < kAtOnce; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = a[e];
-                x[4 + e] = b[e];
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (kLoads == 1) x[u][e] = static_cast<float>(as_half8(raw[u][0])[e]);
+                else x[u][e] = as_float4(raw[u][e / 4])[e & 3];
+            }
+        if (w0 + kAtOnce * kWave < words) request(w0 + kAtOnce * kWave);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int w = w0 + kWave * u + lane;
+            float least = x[u][0], most = x[u][0];
+            uint32_t size = 0;  // (as an integer: NaN is the largest)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                least = fminf(least, x[u][e]);
+                most = fmaxf(most, x[u][e]);
+                size = max(size, __float_as_uint(x[u][e]) << 1);
+            }
+            least = quad_min(least);
+            most = quad_max(most);
+            const int bad = quad_or(size > (__float_as_uint(32768.0f) << 1) ? 1 : 0);
+            const half_t low16 = static_cast<half_t>(least), scale16 = static_cast<half_t>(fifteenth(most - least));
+            uint32_t word = 0, pair = 0x7E000000u;
+            if (!bad) {
+                word = codes_of(x[u], static_cast<float>(low16), static_cast<float>(scale16));
+                pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, scale16)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, low16)) << 16;
+            }
+            // (a row's words are whole groups, so a group's four lanes are all within or all beyond it)
+            if (w < words) {
+                const int head = w >> shift, in_head = w & (per_head - 1);
+                const size_t at = base + static_cast<size_t>(head) * seq_len;
+                codes[at * per_head + in_head] = word;
+                if ((w & 3) == 0) scales[at * (per_head / 4) + in_head / 4] = pair;
             }
         }
-        float least = x[0], most = x[0];
-        int bad = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            least = fminf(least, x[e]);
-            most = fmaxf(most, x[e]);
-            bad |= fabsf(x[e]) <= 32768.0f ? 0 : 1;
-        }
-        least = quad_min(least);
-        most = quad_max(most);
-        bad = quad_or(bad);
-        // (a row's words are whole groups, so a group's four lanes are all here)
-        const half_t low16 = static_cast<half_t>(least), scale16 = static_cast<half_t>((most - least) / 15.0f);
-        const float low = static_cast<float>(low16), scale = static_cast<float>(scale16);
-        const float inverse = scale > 0.0f ? 1.0f / scale : 0.0f;
-        uint32_t word = 0, pair = 0x7E000000u;
-        if (!bad) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) word |= code_of(x[e], low, scale, inverse) << (4 * (e / 2) + 16 * (e & 1));
-            pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, scale16)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, low16)) << 16;
-        }
-        const int head = w / per_head, in_head = w - head * per_head;
-        const size_t at = (static_cast<size_t>(s) * n_kv_heads + head) * seq_len + static_cast<size_t>(pos);
-        codes[at * per_head + in_head] = word;
-        if ((w & 3) == 0) scales[at * (per_head / 4) + in_head / 4] = pair;
     }
 }
 
@@ -131,106 +172,195 @@ __device__ __forceinline__ uint32_t key_of(float mass) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// One workgroup per sequence and KV head: the keep - recent positions of largest weight among the first n - recent, by the bits of the
-// smallest one kept, eight at a time from the top (256 counts a pass), then the list in order.
+// Sum over the wavefront's lanes up to and with this one.
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr by 1, 2, 4, 8: zero comes in
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+    const int row = lane_id() >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+
+// One workgroup per sequence and KV head: the keep - recent positions of largest weight among the first n - recent, then the list in order.
+// The smallest weight kept is found by its bits, 11, 11 and 10 at a time from the top: counts of every value of those bits among the weights
+// that agree with what is known, added up from above.  A thread holds kHeld weights in registers (kOnce: all it has; else
+// stretches of them, read again in every pass).
+constexpr int kBins = 2048;
+template <int kHeld, bool kOnce>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(int* __restrict__ kept, int* __restrict__ dst_lengths, const float* __restrict__ mass,
                                                                 const int* __restrict__ lengths, int n_kv_heads, int seq_len, int keep, int recent) {
-    __shared__ int counts[256];
-    __shared__ int wave_counts[2][kSelectWaves];
+    constexpr int kStretch = kHeld * kSelectThreads, kPerThread = kBins / kSelectThreads;
+    __shared__ int counts[kBins];
+    __shared__ int wave_counts[kHeld * kSelectWaves], wave_equals[kHeld * kSelectWaves];
+    __shared__ int wave_sums[kSelectWaves];
     __shared__ int found_bin, found_above;
-    const int plane = blockIdx.x, s = plane / n_kv_heads, lane = lane_id(), wave = wave_index();
+    const int plane = blockIdx.x, s = plane / n_kv_heads, lane = lane_id(), wave = wave_index(), thread = threadIdx.x;
     const int n = min(max(lengths[s], 0), seq_len), most = min(n, keep);
     int* list = kept + static_cast<size_t>(plane) * keep;
     const float* m = mass + static_cast<size_t>(plane) * seq_len;
-    if (plane % n_kv_heads == 0 && threadIdx.x == 0) dst_lengths[s] = most;
-    for (int i = most + threadIdx.x; i < keep; i += kSelectThreads) list[i] = -1;
+    if (plane % n_kv_heads == 0 && thread == 0) dst_lengths[s] = most;
+    for (int i = most + thread; i < keep; i += kSelectThreads) list[i] = -1;
     if (n <= keep) {
-        for (int i = threadIdx.x; i < n; i += kSelectThreads) list[i] = i;
+        for (int i = thread; i < n; i += kSelectThreads) list[i] = i;
         return;
     }
     const int others = n - recent, want = keep - recent;  // (others > want >= 0)
-    for (int i = threadIdx.x; i < recent; i += kSelectThreads) list[want + i] = others + i;
+    for (int i = thread; i < recent; i += kSelectThreads) list[want + i] = others + i;
     if (want == 0) return;
+    uint32_t keys[kHeld];
+    auto read = [&](int base) {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int i = base + j * kSelectThreads + thread;
+            keys[j] = __float_as_uint(m[min(i, others - 1)]);
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) keys[j] = key_of(__uint_as_float(keys[j]));
+    };
+    // (positions at or behind `others` are those whose number says so)
+    if constexpr (kOnce) read(0);
     uint32_t prefix = 0, mask = 0;
     int still = want;  // of those whose upper bits are `prefix`, how many are kept
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kSelectThreads) counts[i] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) counts[i * kSelectThreads + thread] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < others; i += kSelectThreads) {
-            const uint32_t key = key_of(m[i]);
-            if ((key & mask) == prefix) atomicAdd(&counts[(key >> shift) & 255], 1);
+        for (int base = 0; base < others; base += kStretch) {
+            if constexpr (!kOnce) read(base);
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                if (base + j * kSelectThreads + thread < others && (keys[j] & mask) == prefix) atomicAdd(&counts[(keys[j] >> shift) & digits], 1);
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int above = 0, bin = 255;
-            while (above + counts[bin] < still) above += counts[bin--];  // (the counts add up to `still` at least)
-            found_bin = bin;
-            found_above = above;
+        // thread t has bins kBins - 1 - kPerThread t and below: sums from above
+        int mine[kPerThread], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            mine[i] = counts[kBins - 1 - kPerThread * thread - i];
+            sum += mine[i];
+        }
+        const int upto = wave_inclusive_sum(sum);
+        if (lane == kWave - 1) wave_sums[wave] = upto;
+        __syncthreads();
+        int above = upto - sum;
+        for (int w = 0; w < wave; ++w) above += wave_sums[w];
+#pragma unroll
+        for (int i = 0; i < kPerThread; ++i) {
+            if (above < still && above + mine[i] >= still) {  // (one bin of one thread)
+                found_bin = kBins - 1 - kPerThread * thread - i;
+                found_above = above;
+            }
+            above += mine[i];
         }
         __syncthreads();
         prefix |= static_cast<uint32_t>(found_bin) << shift;
-        mask |= 255u << shift;
+        mask |= digits << shift;
         still -= found_above;
-        __syncthreads();
+        // (found_bin is written again after two barriers)
     }
-    // `prefix` is the smallest weight kept; of those that have it, the first `still` positions.
+    // `prefix` is the smallest weight kept; of those that have it, the first `still` positions.  Counts of every 64 positions, added up in order.
     int kept_before = 0, equal_before = 0;
-    for (int base = 0; base < others; base += kSelectThreads) {
-        const int i = base + threadIdx.x;
-        const uint32_t key = i < others ? key_of(m[i]) : 0u;
-        const bool over = i < others && key > prefix, equal = i < others && key == prefix;
-        const unsigned long long below = (1ull << lane) - 1ull;
-        const unsigned long long overs = __builtin_amdgcn_ballot_w64(over), equals = __builtin_amdgcn_ballot_w64(equal);
-        if (lane == 0) {
-            wave_counts[0][wave] = __popcll(overs);
-            wave_counts[1][wave] = __popcll(equals);
+    const unsigned long long below = (1ull << lane) - 1ull;
+    for (int base = 0; base < others; base += kStretch) {
+        if constexpr (!kOnce) read(base);
+        unsigned long long overs[kHeld], equals[kHeld];
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const bool there = base + j * kSelectThreads + thread < others;
+            overs[j] = __builtin_amdgcn_ballot_w64(there && keys[j] > prefix);
+            equals[j] = __builtin_amdgcn_ballot_w64(there && keys[j] == prefix);
+            if (lane == 0) {
+                wave_counts[j * kSelectWaves + wave] = __popcll(overs[j]);
+                wave_equals[j * kSelectWaves + wave] = __popcll(equals[j]);
+            }
         }
         __syncthreads();
-        int over_at = 0, equal_at = equal_before, over_all = 0, equal_all = 0;
-        for (int w = 0; w < kSelectWaves; ++w) {
-            if (w < wave) {
-                over_at += wave_counts[0][w];
-                equal_at += wave_counts[1][w];
+        // every wavefront adds all of them up by itself, 64 at a time, and keeps what is before its own
+        int over_at[kHeld], equal_at[kHeld], over_all = 0, equal_all = 0;
+#pragma unroll
+        for (int j0 = 0; j0 < kHeld; j0 += kWave / kSelectWaves) {
+            const int at = j0 * kSelectWaves + lane;
+            const int over = at < kHeld * kSelectWaves ? wave_counts[at] : 0, equal = at < kHeld * kSelectWaves ? wave_equals[at] : 0;
+            const int over_upto = wave_inclusive_sum(over), equal_upto = wave_inclusive_sum(equal);
+#pragma unroll
+            for (int j = j0; j < j0 + kWave / kSelectWaves && j < kHeld; ++j) {
+                const int me = (j - j0) * kSelectWaves + wave;
+                over_at[j] = over_all + __builtin_amdgcn_readlane(over_upto - over, me);
+                equal_at[j] = equal_all + __builtin_amdgcn_readlane(equal_upto - equal, me);
             }
-            over_all += wave_counts[0][w];
-            equal_all += wave_counts[1][w];
+            over_all += __builtin_amdgcn_readlane(over_upto, kWave - 1);
+            equal_all += __builtin_amdgcn_readlane(equal_upto, kWave - 1);
         }
-        over_at += __popcll(overs & below);
-        equal_at += __popcll(equals & below);
-        // before position i: over_at larger ones in this stretch, and as many equal ones as are kept
-        const int equal_kept_here = min(equal_at, still) - min(equal_before, still);
-        if (over || (equal && equal_at < still)) list[kept_before + over_at + equal_kept_here] = i;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int equal_rank = equal_before + equal_at[j] + __popcll(equals[j] & below);
+            const int at = kept_before + over_at[j] + __popcll(overs[j] & below) + min(equal_rank, still) - min(equal_before, still);
+            const bool over = (overs[j] >> lane) & 1ull, equal = (equals[j] >> lane) & 1ull;
+            if (over || (equal && equal_rank < still)) list[at] = base + j * kSelectThreads + thread;
+        }
         kept_before += over_all + min(equal_before + equal_all, still) - min(equal_before, still);
         equal_before += equal_all;
-        __syncthreads();
+        if constexpr (!kOnce) __syncthreads();
     }
 }
 
-// Rows of the list, 16 bytes a thread: per row head_size / 32 pieces of K codes, as many of V codes, then one thread each for the
-// scales of K and V and the weight.  blockIdx.y: sequences and KV heads.
-constexpr int kMoveThreads = 256;
+// Rows of the list.  A block has kMovePieces pieces of one part of the cache, one behind the other: 16 bytes of codes of K or V (first
+// blocks, `code_blocks` each), or a row's scales of K and V and its weight.  blockIdx.y: sequences and KV heads.
+constexpr int kMoveThreads = 256, kMoveEach = 4, kMovePieces = kMoveThreads * kMoveEach;
 template <int kHs>
 __global__ __launch_bounds__(kMoveThreads) void move_kernel(Kv4Layer to, float* __restrict__ to_mass, const int* __restrict__ kept, Kv4Layer from,
-                                                            const float* __restrict__ from_mass, int planes, int to_len, int from_len, int keep) {
-    constexpr int kPieces = kHs / 32;
-    const long long i = static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x;
-    const int row = static_cast<int>(i / (2 * kPieces + 2)), piece = static_cast<int>(i % (2 * kPieces + 2));
-    if (row >= to_len) return;
+                                                            const float* __restrict__ from_mass, int planes, int to_len, int from_len, int keep,
+                                                            int code_blocks) {
+    constexpr unsigned kCodes = kHs / 32, kWords = kHs / kKv4Group;
+    typedef uint32_t Scales __attribute__((ext_vector_type(kWords)));
+    const int block = blockIdx.x;
     for (int plane = blockIdx.y; plane < planes; plane += gridDim.y) {
-        const int source = row < keep ? kept[static_cast<size_t>(plane) * keep + row] : -1;
-        const size_t dst = static_cast<size_t>(plane) * to_len + row;
-        if (source < 0) {
-            if (piece == 0) to_mass[dst] = 0.0f;
-            continue;
-        }
-        const size_t src = static_cast<size_t>(plane) * from_len + source;
-        if (piece < 2 * kPieces) {
-            const int which = piece / kPieces, part = piece % kPieces;
-            reinterpret_cast<uintx4*>(to.codes[which])[dst * kPieces + part] = reinterpret_cast<const uintx4*>(from.codes[which])[src * kPieces + part];
-            if (piece == 0) to_mass[dst] = from_mass[src];
+        const size_t dst = static_cast<size_t>(plane) * to_len, src = static_cast<size_t>(plane) * from_len;
+        const int* list = kept + static_cast<size_t>(plane) * keep;
+        int source[kMoveEach];
+        if (block < 2 * code_blocks) {
+            const int which = block >= code_blocks;
+            const unsigned first = static_cast<unsigned>(which ? block - code_blocks : block) * kMovePieces + threadIdx.x;
+            const uintx4* in = reinterpret_cast<const uintx4*>(from.codes[which]) + src * kCodes;
+            uintx4* out = reinterpret_cast<uintx4*>(to.codes[which]) + dst * kCodes;
+            uintx4 x[kMoveEach];
+#pragma unroll
+            for (int u = 0; u < kMoveEach; ++u) {
+                const unsigned row = (first + kMoveThreads * u) / kCodes;
+                source[u] = row < static_cast<unsigned>(keep) ? list[row] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < kMoveEach; ++u) x[u] = in[static_cast<size_t>(max(source[u], 0)) * kCodes + (first + kMoveThreads * u) % kCodes];
+#pragma unroll
+            for (int u = 0; u < kMoveEach; ++u)
+                if (source[u] >= 0) out[first + kMoveThreads * u] = x[u];
         } else {
-            const int which = piece - 2 * kPieces;
-            for (int g = 0; g < kPieces; ++g) to.scales[which][dst * kPieces + g] = from.scales[which][src * kPieces + g];
+            const unsigned first = static_cast<unsigned>(block - 2 * code_blocks) * kMovePieces + threadIdx.x;
+            Scales x[2][kMoveEach];
+            float w[kMoveEach];
+#pragma unroll
+            for (int u = 0; u < kMoveEach; ++u) source[u] = first + kMoveThreads * u < static_cast<unsigned>(keep) ? list[first + kMoveThreads * u] : -1;
+#pragma unroll
+            for (int u = 0; u < kMoveEach; ++u) {
+                const size_t at = src + max(source[u], 0);
+                x[0][u] = reinterpret_cast<const Scales*>(from.scales[0])[at];
+                x[1][u] = reinterpret_cast<const Scales*>(from.scales[1])[at];
+                w[u] = from_mass[at];
+            }
+#pragma unroll
+            for (int u = 0; u < kMoveEach; ++u) {
+                const unsigned row = first + kMoveThreads * u;
+                if (source[u] >= 0) {
+                    reinterpret_cast<Scales*>(to.scales[0])[dst + row] = x[0][u];
+                    reinterpret_cast<Scales*>(to.scales[1])[dst + row] = x[1][u];
+                }
+                if (row < static_cast<unsigned>(to_len)) to_mass[dst + row] = source[u] >= 0 ? w[u] : 0.0f;
+            }
         }
     }
 }
@@ -319,18 +449,19 @@ lpp_status lpp_kv4_evict(void* d_dst, const lpp_kv4_shape* dst, int dst_layer, f
                 "lpp_kv4_evict: d_dst_lengths overlaps d_lengths");
     float* dst_mass = d_dst_mass + kv4_layer_rows(*dst) * dst_layer;
     const float* src_mass = d_mass + kv4_layer_rows(*src) * src_layer;
-    hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(planes)), dim3(kSelectThreads), 0, stream(), d_kept, d_dst_lengths, src_mass, d_lengths,
+    const auto select = src->seq_len <= 4 * kSelectThreads    ? &select_kernel<4, true>
+                        : src->seq_len <= 8 * kSelectThreads  ? &select_kernel<8, true>
+                        : src->seq_len <= 32 * kSelectThreads ? &select_kernel<32, true>
+                                                              : &select_kernel<32, false>;
+    hipLaunchKernelGGL(select, dim3(static_cast<unsigned>(planes)), dim3(kSelectThreads), 0, stream(), d_kept, d_dst_lengths, src_mass, d_lengths,
                        dst->n_kv_heads, src->seq_len, keep, recent);
     LPP_CHECK_LAUNCH("select_kernel");
     const Kv4Layer to = kv4_layer(d_dst, *dst, dst_layer), from = kv4_layer(d_src, *src, src_layer);
-    const long long threads = static_cast<long long>(dst->seq_len) * (2 * dst->head_size / 32 + 2);
-    const dim3 grid(static_cast<unsigned>((threads + kMoveThreads - 1) / kMoveThreads), static_cast<unsigned>(planes < 65535 ? planes : 65535));
-    if (dst->head_size == 64)
-        hipLaunchKernelGGL((move_kernel<64>), grid, dim3(kMoveThreads), 0, stream(), to, dst_mass, d_kept, from, src_mass, static_cast<int>(planes),
-                           dst->seq_len, src->seq_len, keep);
-    else
-        hipLaunchKernelGGL((move_kernel<128>), grid, dim3(kMoveThreads), 0, stream(), to, dst_mass, d_kept, from, src_mass, static_cast<int>(planes),
-                           dst->seq_len, src->seq_len, keep);
+    const auto blocks_of = [](long long pieces) { return static_cast<int>((pieces + kMovePieces - 1) / kMovePieces); };
+    const int code_blocks = blocks_of(static_cast<long long>(keep) * (dst->head_size / 32));
+    const dim3 grid(2 * code_blocks + blocks_of(dst->seq_len), static_cast<unsigned>(planes < 65535 ? planes : 65535));
+    hipLaunchKernelGGL((dst->head_size == 64 ? &move_kernel<64> : &move_kernel<128>), grid, dim3(kMoveThreads), 0, stream(), to, dst_mass, d_kept, from,
+                       src_mass, static_cast<int>(planes), dst->seq_len, src->seq_len, keep, code_blocks);
     LPP_CHECK_LAUNCH("move_kernel");
     return LPP_OK;
 }

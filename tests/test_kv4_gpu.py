@@ -411,7 +411,7 @@ def evict(lib, cache, mass, lengths, keep, recent, room, layer=0, dst_layers=1, 
 @pytest.mark.parametrize("hs,kv", [(64, 2), (128, 3)])
 @pytest.mark.parametrize("lengths,keep,recent,room", [
     ([1], 1, 0, 1), ([5, 0, 9], 4, 2, 4), ([100, 64, 3], 64, 64, 70), ([1024, 1025, 2047], 300, 0, 300), ([1500, -4, 9999], 1, 1, 5),
-    ([1500, 1499, 700], 1499, 10, 1499), ([3000], 999, 33, 1200), ([5000], 4000, 17, 4001), ([20000], 77, 5, 80)], ids=str)
+    ([1500, 1499, 700], 1499, 10, 1499), ([3000], 999, 33, 1200), ([5000], 4000, 17, 4001), ([20000], 77, 5, 80), ([40000, 70000], 36000, 100, 36000)], ids=str)
 def test_evict(lib, lengths, keep, recent, room, hs, kv):
     rng = np.random.default_rng(keep + hs)
     full = max(max(lengths), 1) if 9999 not in lengths else 1500
