@@ -85,19 +85,5 @@ struct Kv4Reader {
     }
 };
 
-// The sequence that has packed row `row`: the number of sequences that end at or before it (n_seqs: none has it).  `ends`
-// does not decrease.  All lanes of the wavefront call it with the same row and look at 64 ends at a time.
-__device__ __forceinline__ int sequence_of_row(const int* __restrict__ ends, int n_seqs, int row) {
-    int before = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += kWave) {
-        const int s = s0 + lane_id();
-        const bool ended = s < n_seqs && ends[s] <= row;
-        const int here = __popcll(__builtin_amdgcn_ballot_w64(ended));
-        before += here;
-        if (here < kWave) break;
-    }
-    return before;
-}
-
 }  // namespace dev
 }  // namespace lpp

@@ -23,28 +23,35 @@ __device__ __forceinline__ int quad_or(int v) {
     return v | dpp_move_i<kDppXor2>(v);
 }
 
-// A word of the codes of eight values: the integers nearest to (x - low) / scale, in 0 .. 15.  In fp32 the quotient, cut to that range, is off by less
-// than 16 * 5 * 2^-24 (difference, reciprocal, product), so a word with a quotient within 1e-5 of a border, one in 6000, is formed
-// again in 64 bits.  Adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the lowest bits: the codes are added up
-// with what is above them, which is taken off at the end.
+// A word of the codes of eight values: the integers nearest to (x - low) / scale, in 0 .. 15.  In fp32, as fifteen times a number that is cut to
+// 0 .. 1 as it is formed, the quotient is off by less than 15 * 4 * 2^-24 and by 2^-22 of low / scale; a word with a quotient nearer than that to a
+// border (within 1e-5 and 2^-21) is formed again by the sign of x - low - border * scale.  (Of fp32 values that is one word in 6000; binary16 values lie
+// on a border itself often, about one word in 300.)  Adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the
+// lowest bits: the codes are added up with what is above them, which is taken off at the end.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float scale) {
     const float inverse = scale > 0.0f ? __builtin_amdgcn_rcpf(scale) : 0.0f;
+    const float slope = inverse * (1.0f / 15.0f), shift = -low * slope;
     uint32_t word = 0, above = 0;
     float furthest = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float t = __builtin_amdgcn_fmed3f((x[e] - low) * inverse, 0.0f, 15.0f), shifted = t + 8388608.0f;
-        furthest = fmaxf(furthest, fabsf(t - (shifted - 8388608.0f)));
+        const float t = __builtin_amdgcn_fmed3f(fmaf(x[e], slope, shift), 0.0f, 1.0f), shifted = fmaf(t, 15.0f, 8388608.0f);
+        furthest = fmaxf(furthest, fabsf(fmaf(t, 15.0f, 8388608.0f - shifted)));
         word += __float_as_uint(shifted) << (4 * (e / 2) + 16 * (e & 1));
         above += 0x4B000000u << (4 * (e / 2) + 16 * (e & 1));
     }
     word -= above;
-    if (furthest > 0.5f - 1e-5f) {
+    if (furthest > 0.5f - 1e-5f - fabsf(low * inverse) * 0x1p-21f) {
+#pragma clang fp contract(off)
         word = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const double t = rint((static_cast<double>(x[e]) - static_cast<double>(low)) / static_cast<double>(scale));
-            word |= static_cast<uint32_t>(fmin(fmax(t, 0.0), 15.0)) << (4 * (e / 2) + 16 * (e & 1));
+            // difference + left is x - low; the border between f and f + 1 (an f one off near an integer decides the same)
+            const float difference = x[e] - low, taken = difference - x[e], left = (x[e] - (difference - taken)) + (-low - taken);
+            const float f = floorf(__builtin_amdgcn_fmed3f(difference * inverse, 0.0f, 14.0f));
+            const float beyond = fmaf(-(f + 0.5f), scale, difference) + left;
+            const uint32_t below = static_cast<uint32_t>(f);
+            word |= (below + (beyond > 0.0f || (beyond == 0.0f && (below & 1u)) ? 1u : 0u)) << (4 * (e / 2) + 16 * (e & 1));
         }
     }
     return word;
@@ -61,83 +68,100 @@ __device__ __forceinline__ float fifteenth(float r) {
     return quotient;
 }
 
-// One wavefront per row of K or V; a lane has a word's eight values, two words at a time.  The first values are requested before anything is
-// known about the row's sequence.
+// One wavefront per row, K and V; a lane has a word's eight values, two words of each at a time.  The first values are requested along with the
+// sequences' ends and starts, before anything is known about the row: what a row takes is the time of its requests, one after the other.
 template <typename T>
 __global__ __launch_bounds__(kStoreThreads) void store_kernel(Kv4Layer to, const T* __restrict__ k, const T* __restrict__ v, int stride,
                                                               const int* __restrict__ offsets, const int* __restrict__ starts, int n_tokens,
                                                               int n_seqs, int n_kv_heads, int head_size, int seq_len) {
     constexpr int kAtOnce = 2, kLoads = sizeof(T) / 2;  // words; requests of 16 bytes to a word
-    const int wave = wave_index(), lane = lane_id();
-    const int row = static_cast<int>(blockIdx.x) * 2 + wave / 2, which = wave & 1;
+    const int lane = lane_id();
+    const int row = static_cast<int>(blockIdx.x) * (kStoreThreads / kWave) + wave_index();
     if (row >= n_tokens) return;
-    const T* from = (which ? v : k) + static_cast<size_t>(row) * stride;
+    const T* from[2] = {k + static_cast<size_t>(row) * stride, v + static_cast<size_t>(row) * stride};
     const int words = n_kv_heads * head_size / 8, per_head = head_size / 8;
-    uintx4 raw[kAtOnce][kLoads];
+    uintx4 raw[2][kAtOnce][kLoads];
     auto request = [&](int w0) {
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const int w = min(w0 + kWave * u + lane, words - 1);
+        for (int which = 0; which < 2; ++which)
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) raw[u][i] = load16(from + 8 * w + 8 / kLoads * i);
-        }
+            for (int u = 0; u < kAtOnce; ++u) {
+                const int w = min(w0 + kWave * u + lane, words - 1);
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) raw[which][u][i] = load16(from[which] + 8 * w + 8 / kLoads * i);
+            }
     };
     request(0);
-    int s, first;
+    int s = 0, first = 0, start = 0;
     if (offsets != nullptr) {
-        s = sequence_of_row(offsets + 1, n_seqs, row);
-        if (s >= n_seqs) return;
-        first = max(offsets[s], 0);
+        int begin = offsets[0];
+        for (;; s += kWave) {
+            if (s >= n_seqs) return;
+            const int at = min(s + lane, n_seqs - 1);
+            const int end = offsets[at + 1], its_start = starts != nullptr ? starts[at] : 0;
+            const int ended = __popcll(__builtin_amdgcn_ballot_w64(end <= row && s + lane < n_seqs));
+            if (ended > 0) begin = __builtin_amdgcn_readlane(end, ended - 1);
+            if (ended == kWave) continue;
+            s += ended;
+            if (s >= n_seqs) return;
+            start = __builtin_amdgcn_readlane(its_start, ended);
+            break;
+        }
+        first = max(begin, 0);
         if (row < first) return;
     } else {
         const int each = n_tokens / n_seqs;
         s = row / each;
         first = s * each;
+        if (starts != nullptr) start = starts[s];
     }
-    const long long pos = (starts != nullptr ? static_cast<long long>(starts[s]) : 0ll) + row - first;
+    const long long pos = static_cast<long long>(start) + row - first;
     if (pos < 0 || pos >= seq_len) return;
-    uint32_t* codes = to.codes[which];
-    uint32_t* scales = to.scales[which];
     const int shift = per_head == 8 ? 3 : 4;
     const size_t base = static_cast<size_t>(s) * n_kv_heads * seq_len + static_cast<size_t>(pos);
     for (int w0 = 0; w0 < words; w0 += kAtOnce * kWave) {
-        float x[kAtOnce][8];
+        float x[2][kAtOnce][8];
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u)
+        for (int which = 0; which < 2; ++which)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (kLoads == 1) x[u][e] = static_cast<float>(as_half8(raw[u][0])[e]);
-                else x[u][e] = as_float4(raw[u][e / 4])[e & 3];
-            }
+            for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if constexpr (kLoads == 1) x[which][u][e] = static_cast<float>(as_half8(raw[which][u][0])[e]);
+                    else x[which][u][e] = as_float4(raw[which][u][e / 4])[e & 3];
+                }
         if (w0 + kAtOnce * kWave < words) request(w0 + kAtOnce * kWave);
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const int w = w0 + kWave * u + lane;
-            float least = x[u][0], most = x[u][0];
-            uint32_t size = 0;  // (as an integer: NaN is the largest)
+        for (int which = 0; which < 2; ++which)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                least = fminf(least, x[u][e]);
-                most = fmaxf(most, x[u][e]);
-                size = max(size, __float_as_uint(x[u][e]) << 1);
+            for (int u = 0; u < kAtOnce; ++u) {
+                const float(&mine)[8] = x[which][u];
+                const int w = w0 + kWave * u + lane;
+                float least = mine[0], most = mine[0];
+                uint32_t size = 0;  // (as an integer: NaN is the largest)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    least = fminf(least, mine[e]);
+                    most = fmaxf(most, mine[e]);
+                    size = max(size, __float_as_uint(mine[e]) << 1);
+                }
+                least = quad_min(least);
+                most = quad_max(most);
+                const int bad = quad_or(size > (__float_as_uint(32768.0f) << 1) ? 1 : 0);
+                const half_t low16 = static_cast<half_t>(least), scale16 = static_cast<half_t>(fifteenth(most - least));
+                uint32_t word = 0, pair = 0x7E000000u;
+                if (!bad) {
+                    word = codes_of(mine, static_cast<float>(low16), static_cast<float>(scale16));
+                    pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, scale16)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, low16)) << 16;
+                }
+                // (a row's words are whole groups, so a group's four lanes are all within or all beyond it)
+                if (w < words) {
+                    const int head = w >> shift, in_head = w & (per_head - 1);
+                    const size_t at = base + static_cast<size_t>(head) * seq_len;
+                    to.codes[which][at * per_head + in_head] = word;
+                    if ((w & 3) == 0) to.scales[which][at * (per_head / 4) + in_head / 4] = pair;
+                }
             }
-            least = quad_min(least);
-            most = quad_max(most);
-            const int bad = quad_or(size > (__float_as_uint(32768.0f) << 1) ? 1 : 0);
-            const half_t low16 = static_cast<half_t>(least), scale16 = static_cast<half_t>(fifteenth(most - least));
-            uint32_t word = 0, pair = 0x7E000000u;
-            if (!bad) {
-                word = codes_of(x[u], static_cast<float>(low16), static_cast<float>(scale16));
-                pair = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, scale16)) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, low16)) << 16;
-            }
-            // (a row's words are whole groups, so a group's four lanes are all within or all beyond it)
-            if (w < words) {
-                const int head = w >> shift, in_head = w & (per_head - 1);
-                const size_t at = base + static_cast<size_t>(head) * seq_len;
-                codes[at * per_head + in_head] = word;
-                if ((w & 3) == 0) scales[at * (per_head / 4) + in_head / 4] = pair;
-            }
-        }
     }
 }
 
@@ -394,7 +418,7 @@ lpp_status lpp_kv4_store(void* d_cache, const lpp_kv4_shape* shape, int layer, c
     LPP_REQUIRE(reinterpret_cast<uintptr_t>(d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(d_v) % 16 == 0 && kv_stride % per16 == 0,
                 "lpp_kv4_store: rows of K and V must start at multiples of 16 bytes");
     const Kv4Layer to = kv4_layer(d_cache, *shape, layer);
-    const dim3 grid((static_cast<unsigned>(n_tokens) + 1) / 2);
+    const dim3 grid((static_cast<unsigned>(n_tokens) + kStoreThreads / dev::kWave - 1) / (kStoreThreads / dev::kWave));
     if (type == LPP_F32)
         hipLaunchKernelGGL((store_kernel<float>), grid, dim3(kStoreThreads), 0, stream(), to, static_cast<const float*>(d_k), static_cast<const float*>(d_v),
                            kv_stride, d_offsets, d_starts, n_tokens, shape->n_seqs, shape->n_kv_heads, shape->head_size, shape->seq_len);
