@@ -471,7 +471,7 @@ enum { LPP_F32 = 0, LPP_F16 = 1 };
  * allowed.  NULL: one sequence of n_tokens rows (n_seqs is 1 then).  Rows of d_out that no sequence has are left as they
  * were.
  * q and out: [n_tokens][n_heads * head_size] of `type`; k and v: binary16 [n_tokens][n_kv_heads * head_size], what the
- * caches hold; the strides are the elements from one row to the next.  Rows start at multiples of 16 bytes.  d_out must
+ * caches hold; the strides are the elements from one row to the next, kv_stride at most 2^24.  Rows start at multiples of 16 bytes.  d_out must
  * not overlap the inputs.  LPP_F32: queries and weights enter the products as binary16 head and remainder, as in
  * LPP_PREFILL_EXACT; LPP_F16: the weights are rounded to binary16 where V is weighted, sums are fp32, the output is rounded
  * once.  What K and V rows hold that a row does not attend to does not reach it, infinities and NaN included. */

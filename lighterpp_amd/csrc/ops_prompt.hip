@@ -1,5 +1,7 @@
 // ops_prompt.hip -- lpp_prompt_attention: causal attention of whole prompts,
 // packed one behind the other.
+#include <type_traits>
+
 #include "kv4.hpp"
 
 namespace lpp {
@@ -125,19 +127,47 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
     char* stages = lds + wp * S::kStages * S::kStageBytes;
     const unsigned lds_base = static_cast<unsigned>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)stages));
     const int steps = (limit + kStep - 1) / kStep, turns = (steps + kP - 1) / kP;
-    constexpr int kRowsPerLoad = 1024 / kRowBytes, kLoadsPerHalf = S::kHalfBytes / 1024;
+    // Requests of 1 KiB, kRowsPerLoad rows each: a wavefront's are kR apart, so that the order of a row's pieces repeats every kKinds of them,
+    // and what a lane adds to a uniform address is the same for those.  Only the last step looks where the rows end (rows behind are the last
+    // one again).
+    constexpr int kRowsPerLoad = 1024 / kRowBytes, kLoadsPerHalf = S::kHalfBytes / 1024, kEach = kLoadsPerHalf / kR;
+    constexpr int kPeriod = kHs == 64 ? 2 : 4, kKinds = kR >= kPeriod ? 1 : kPeriod / kR;
+    auto k_order = [](int row) { return kHs == 64 ? (row >> 1) & 7 : row & 15; };
+    auto v_order = [](int row) { return kHs == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3); };
+    const uint32_t row_step32 = static_cast<uint32_t>(row_step);
+    uint32_t k_off[kKinds];
+#pragma unroll
+    for (int i = 0; i < kKinds; ++i) {
+        const int row = (wr + kR * i) * kRowsPerLoad + lane / kPieces;
+        k_off[i] = lane / kPieces * row_step32 + 16 * ((lane % kPieces) ^ k_order(row));
+    }
+    const uint32_t v_off = lane / kPieces * row_step32 + 16 * ((lane % kPieces) ^ v_order(lane / kPieces));
+    auto load_lds = [](const char* base, uint32_t offset, unsigned at) {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n" ::"v"(offset), "s"(base), "s"(at) : "memory");
+    };
     auto request = [&](int turn) {
         const int p0 = (turn * kP + wp) * kStep;
+        if (p0 >= limit) return;  // (one row of wavefronts: never)
+        const unsigned at = __builtin_amdgcn_readfirstlane(lds_base + (turn % S::kStages) * S::kStageBytes);
+        if (p0 + kStep <= limit) {
 #pragma unroll
-        for (int i = 0; i < S::kRequests; ++i) {
-            const int load = wr + kR * i, in_half = load % kLoadsPerHalf;
-            const bool is_v = load >= kLoadsPerHalf;  // (uniform)
-            const int row = in_half * kRowsPerLoad + lane / kPieces;
-            const int swizzle = is_v ? (kHs == 64 ? 4 * ((row >> 1) & 1) : 4 * (row & 3)) : (kHs == 64 ? (row >> 1) & 7 : row & 15);
-            const int pos = min(p0 + row, limit - 1);
-            const char* src = (is_v ? vbase : kbase) + static_cast<size_t>(pos) * row_step + 16 * ((lane % kPieces) ^ swizzle);
-            const unsigned at = __builtin_amdgcn_readfirstlane(lds_base + (turn % S::kStages) * S::kStageBytes + load * 1024);
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off\n" ::"v"(src), "s"(at) : "memory");
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) {
+                    const int load = wr + kR * i;
+                    const char* base = (w ? vbase : kbase) + static_cast<size_t>(p0 + load * kRowsPerLoad) * row_step;
+                    load_lds(base, w ? v_off : k_off[i % kKinds], at + w * S::kHalfBytes + load * 1024);
+                }
+        } else {
+            const char* base[2] = {kbase + static_cast<size_t>(p0) * row_step, vbase + static_cast<size_t>(p0) * row_step};
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int load = wr + kR * i, row = load * kRowsPerLoad + lane / kPieces;
+                const uint32_t off = static_cast<uint32_t>(min(row, limit - 1 - p0)) * row_step32;
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+                    load_lds(base[w], off + 16 * ((lane % kPieces) ^ (w ? v_order(row) : k_order(row))), at + w * S::kHalfBytes + load * 1024);
+            }
         }
     };
     request(0);
@@ -187,15 +217,9 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
         }
     }
 
-    for (int turn = 0; turn < turns; ++turn) {
-        const int p0 = (turn * kP + wp) * kStep;
-        // (the step's rows have landed, and nobody reads the stage the next requests go to any more)
-        wait_requests<0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if constexpr (kR > 1) __syncthreads();
-        if (turn + 1 < turns) request(turn + 1);
-        if (p0 >= wave_limit) continue;
-        const char* stage = stages + (turn % S::kStages) * S::kStageBytes;
+    // One step: kPartly: some row of the wavefront does not attend to all of it (the last step or two of a walk).
+    auto walk = [&](auto partly, int p0, const char* stage) {
+        constexpr bool kPartly = decltype(partly)::value;
         const char* values = stage + S::kHalfBytes;
         floatx16 st[kTiles];
 #pragma unroll
@@ -209,8 +233,7 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
                 if constexpr (kLo) st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[s], st[t], 0, 0, 0);
             }
         }
-        const bool partly = p0 + kStep > t0 + 1;  // (uniform) some row of the wavefront does not attend to the whole step
-        if (partly) {
+        if constexpr (kPartly) {
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -246,7 +269,6 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
             for (int e = 0; e < 8; e += 2) {
                 const float s_0 = st[s2 >> 1][8 * (s2 & 1) + e], s_1 = st[s2 >> 1][8 * (s2 & 1) + e + 1];
                 float p_0 = __builtin_amdgcn_exp2f(fmaf(s_0, scale, -top)), p_1 = __builtin_amdgcn_exp2f(fmaf(s_1, scale, -top));
-                step_sum += p_0 + p_1;
                 // (the packed pair and the factor -1 are hidden from the compiler, which would otherwise round every value a second time to
                 // subtract it)
                 uint32_t packed = __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(p_0), static_cast<half_t>(p_1)});
@@ -255,8 +277,12 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
                 ph[e] = h[0];
                 ph[e + 1] = h[1];
                 if constexpr (kLo) {
+                    step_sum += p_0 + p_1;
                     pl[e] = static_cast<half_t>(fmaf(static_cast<float>(h[0]), minus_one, p_0));
                     pl[e + 1] = static_cast<half_t>(fmaf(static_cast<float>(h[1]), minus_one, p_1));
+                } else {
+                    // (the sum of the rounded weights, which are what V is weighted with, two to an instruction)
+                    step_sum = __builtin_amdgcn_fdot2(h, half2_t{static_cast<half_t>(1.0f), static_cast<half_t>(1.0f)}, step_sum, false);
                 }
             }
 #pragma unroll
@@ -269,26 +295,39 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
                 for (int j = 0; j < 2; ++j)
                     vf.part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                         (__attribute__((address_space(3))) short4_t*)(values + v_at[dt] + (16 * s2 + 8 * j) * kRowBytes));
-                if (partly && __builtin_amdgcn_ballot_w64(has_nonfinite(vf.whole)) != 0ull) {
-                    // (uniform) An infinity or NaN among V rows that some row does not attend to: a weight of zero would not keep it out.  One
-                    // token after the other, with the rows behind it cleared; a lane's output is its own token's.
-                    for (int token = 0; token < tokens_per_wave; ++token) {
-                        const int end = t0 + token + 1 - p0 - 16 * s2 - 4 * g;  // positions 0..3 and 8..11 from here are this lane's
-                        half8_t seen_v = vf.whole;
+                if constexpr (kPartly) {
+                    if (__builtin_amdgcn_ballot_w64(has_nonfinite(vf.whole)) != 0ull) {
+                        // (uniform) An infinity or NaN among V rows that some row does not attend to: a weight of zero would not keep it out.
+                        // One token after the other, with the rows behind it cleared; a lane's output is its own token's.
+                        for (int token = 0; token < tokens_per_wave; ++token) {
+                            const int end = t0 + token + 1 - p0 - 16 * s2 - 4 * g;  // positions 0..3 and 8..11 from here are this lane's
+                            half8_t seen_v = vf.whole;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if ((e & 3) + 8 * (e >> 2) >= end) seen_v[e] = static_cast<half_t>(0.0f);
-                        floatx16 with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, ph, o[dt], 0, 0, 0);
-                        if constexpr (kLo) with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
-                        if (r / job.shared == token) o[dt] = with;
+                            for (int e = 0; e < 8; ++e)
+                                if ((e & 3) + 8 * (e >> 2) >= end) seen_v[e] = static_cast<half_t>(0.0f);
+                            floatx16 with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, ph, o[dt], 0, 0, 0);
+                            if constexpr (kLo) with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
+                            if (my_tok == t0 + token) o[dt] = with;
+                        }
+                        continue;
                     }
-                } else {
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, ph, o[dt], 0, 0, 0);
-                    if constexpr (kLo) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, pl, o[dt], 0, 0, 0);
                 }
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, ph, o[dt], 0, 0, 0);
+                if constexpr (kLo) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, pl, o[dt], 0, 0, 0);
             }
         }
         lsum += step_sum;
+    };
+    for (int turn = 0; turn < turns; ++turn) {
+        const int p0 = (turn * kP + wp) * kStep;
+        // (the step's rows have landed, and nobody reads the stage the next requests go to any more)
+        wait_requests<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (kR > 1) __syncthreads();
+        if (turn + 1 < turns) request(turn + 1);
+        const char* stage = stages + (turn % S::kStages) * S::kStageBytes;
+        if (p0 + kStep <= t0 + 1) walk(std::false_type{}, p0, stage);  // (uniform)
+        else if (p0 < wave_limit) walk(std::true_type{}, p0, stage);
     }
     lsum = halves_sum(lsum);
     T* out_row = static_cast<T*>(job.out) + static_cast<size_t>(first_row + tok_c) * job.out_stride + (kvh * job.shared + my_head) * kHs + 4 * g;
@@ -405,6 +444,7 @@ lpp_status lpp_prompt_attention(void* d_out, const void* d_q, const lpp_half* d_
     const long long width = static_cast<long long>(n_heads) * head_size, kv_width = static_cast<long long>(n_kv_heads) * head_size;
     LPP_REQUIRE(q_stride >= width && out_stride >= width && kv_stride >= kv_width,
                 "lpp_prompt_attention: strides of %d (q), %d (k, v), %d (out) for rows of %lld and %lld", q_stride, kv_stride, out_stride, width, kv_width);
+    LPP_REQUIRE(kv_stride <= 1 << 24, "lpp_prompt_attention: kv_stride = %d is beyond 2^24", kv_stride);
     if (n_tokens == 0) return LPP_OK;
     LPP_REQUIRE(d_out && d_q && d_k && d_v, "lpp_prompt_attention: null pointer");
     const int size = type == LPP_F32 ? 4 : 2, per16 = 16 / size;

@@ -144,6 +144,7 @@ def test_prompt_refused(lib):
         refused(lib, call(**{name: 258}), b"16 bytes")
     refused(lib, call(sk=127), b"strides")
     refused(lib, call(sk=132), b"16 bytes")
+    refused(lib, call(sk=(1 << 24) + 8), b"kv_stride")
     refused(lib, call(out=2 * P + 1024), b"overlap")
     refused(lib, call(out=4 * P - 16), b"overlap")
 
