@@ -19,7 +19,6 @@ template <int kHs, int kR, int kP, int kStepRows>
 struct Shape {
     static constexpr int kStep = kStepRows, kRowBytes = 2 * kHs, kPieces = kHs / 8;
     static constexpr int kHalfBytes = kStep * kRowBytes, kStageBytes = 2 * kHalfBytes;  // K rows, then V rows
-    static constexpr int kRequests = kStageBytes / 1024 / kR;                           // a wavefront's, of a step
     static constexpr int kStages = 2;
     static constexpr int kPartFloats = (kHs / 2 + 2) * 64;  // a wavefront's maximum, sum and output
     static constexpr int kMergeBytes = kP > 1 ? kP * kR * kPartFloats * 4 : 0;
@@ -61,8 +60,11 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
     return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
 }
 
-// The sequence that tile `tile` of all sequences' tiles is in, one behind the other, and which of its tiles: the last one first, so that the
-// longest walks of a sequence begin first.  Returns the sequence's rows, 0: there are not as many tiles.
+__device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_readlane(wave_inclusive_sum(v), kWave - 1); }
+
+// The `tile`-th of all sequences' tiles: which of its sequence's tiles it is, and the sequence's rows (returned; 0: there are not as many
+// tiles).  Up to 64 sequences: in the order of their walks' lengths, longest first, whatever the sequence; more: one sequence
+// after the other, each from its last tile.
 __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& tile, int& first_row) {
     if (job.offsets == nullptr) {
         first_row = 0;
@@ -75,6 +77,26 @@ __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& 
         const int begin = s < job.n_seqs ? min(max(job.offsets[s], 0), job.n_tokens) : 0;
         const int end = s < job.n_seqs ? min(max(job.offsets[s + 1], 0), job.n_tokens) : 0;
         const int rows = max(end - begin, 0), tiles = (rows + tokens - 1) / tokens;
+        if (job.n_seqs <= kWave) {
+            // tile number `level` of every sequence that has one, from the highest level down: the level with as many tiles above it as
+            // are before this one
+            if (wave_sum_int(tiles) <= tile) return 0;
+            int low = 0, high = static_cast<int>(wave_max(static_cast<float>(min(tiles, 1 << 24))));  // at and above `low` more tiles than `tile`, at `high` not
+            if (high == 1 << 24) high = (job.n_tokens + tokens - 1) / tokens;
+            while (high - low > 1) {
+                const int middle = (low + high) / 2;
+                if (wave_sum_int(max(tiles - middle, 0)) > tile) low = middle;
+                else high = middle;
+            }
+            const int rank = tile - wave_sum_int(max(tiles - low - 1, 0));
+            const unsigned long long there = __builtin_amdgcn_ballot_w64(tiles > low);
+            const int before = __popcll(there & ((1ull << lane) - 1ull));
+            const unsigned long long mine = __builtin_amdgcn_ballot_w64(tiles > low && before == rank);
+            const int at = __builtin_ctzll(mine);
+            first_row = __builtin_amdgcn_readlane(begin, at);
+            tile = low;
+            return __builtin_amdgcn_readlane(rows, at);
+        }
         const int upto = wave_inclusive_sum(tiles);
         const unsigned long long behind = __builtin_amdgcn_ballot_w64(upto > tile);
         if (behind != 0ull) {
@@ -86,14 +108,6 @@ __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& 
         tile -= __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     return 0;
-}
-
-__device__ __forceinline__ bool has_nonfinite(half8_t v) {
-    const uintx4 u = __builtin_bit_cast(uintx4, v);
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) any |= (u[i] & 0x7FFF7FFFu) + 0x04000400u;  // (the exponent's carry)
-    return (any & 0x80008000u) != 0u;
 }
 
 template <typename T, int kHs, int kR, int kP, int kStepRows>
@@ -217,10 +231,11 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
         }
     }
 
-    // One step: kPartly: some row of the wavefront does not attend to all of it (the last step or two of a walk).
-    auto walk = [&](auto partly, int p0, const char* stage) {
+    // `count` tiles of 32 positions from p0 on, K rows at `keys`, V rows at `values`.  kPartly: some row of the wavefront does not attend to all of
+    // them (the last tiles of a walk).
+    auto walk = [&](auto partly, auto count, int p0, const char* keys, const char* values) {
         constexpr bool kPartly = decltype(partly)::value;
-        const char* values = stage + S::kHalfBytes;
+        constexpr int kTiles = decltype(count)::value;
         floatx16 st[kTiles];
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
@@ -228,7 +243,7 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
             for (int e = 0; e < 16; ++e) st[t][e] = 0.0f;
 #pragma unroll
             for (int s = 0; s < kKSteps; ++s) {
-                const half8_t kf = *reinterpret_cast<const half8_t*>(stage + t * 32 * kRowBytes + k_at[s]);
+                const half8_t kf = *reinterpret_cast<const half8_t*>(keys + t * 32 * kRowBytes + k_at[s]);
                 st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qh[s], st[t], 0, 0, 0);
                 if constexpr (kLo) st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[s], st[t], 0, 0, 0);
             }
@@ -261,6 +276,30 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
                 for (int e = 0; e < 16; ++e) o[dt][e] *= corr;
             seen = seen || moves;
         }
+        auto values_of = [&](int s2, int dt) {
+            union {
+                short4_t part[2];
+                half8_t whole;
+            } vf;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                vf.part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) short4_t*)(values + v_at[dt] + (16 * s2 + 8 * j) * kRowBytes));
+            return vf.whole;
+        };
+        bool odd = false;  // an infinity or NaN among V rows that some row may not attend to
+        if constexpr (kPartly) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int s2 = 0; s2 < 2 * kTiles; ++s2)
+#pragma unroll
+                for (int dt = 0; dt < kDTiles; ++dt) {
+                    const uintx4 u = __builtin_bit_cast(uintx4, values_of(s2, dt));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) any |= (u[i] & 0x7FFF7FFFu) + 0x04000400u;  // (the exponent's carry)
+                }
+            odd = __builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0u) != 0ull;
+        }
         float step_sum = 0.0f;  // (of its own, so that the running sum is rounded once a step)
 #pragma unroll
         for (int s2 = 0; s2 < 2 * kTiles; ++s2) {
@@ -285,35 +324,29 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
                     step_sum = __builtin_amdgcn_fdot2(h, half2_t{static_cast<half_t>(1.0f), static_cast<half_t>(1.0f)}, step_sum, false);
                 }
             }
+if (kPartly && odd) {
+                // (uniform) A weight of zero would not keep it out.  One token after the other, with the rows behind it cleared; a lane's output is
+                // its own token's.
+                for (int token = 0; token < tokens_per_wave; ++token) {
+                    const int end = t0 + token + 1 - p0 - 16 * s2 - 4 * g;  // positions 0..3 and 8..11 from here are this lane's
 #pragma unroll
-            for (int dt = 0; dt < kDTiles; ++dt) {
-                union {
-                    short4_t part[2];
-                    half8_t whole;
-                } vf;
+                    for (int dt = 0; dt < kDTiles; ++dt) {
+                        half8_t seen_v = values_of(s2, dt);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    vf.part[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) short4_t*)(values + v_at[dt] + (16 * s2 + 8 * j) * kRowBytes));
-                if constexpr (kPartly) {
-                    if (__builtin_amdgcn_ballot_w64(has_nonfinite(vf.whole)) != 0ull) {
-                        // (uniform) An infinity or NaN among V rows that some row does not attend to: a weight of zero would not keep it out.
-                        // One token after the other, with the rows behind it cleared; a lane's output is its own token's.
-                        for (int token = 0; token < tokens_per_wave; ++token) {
-                            const int end = t0 + token + 1 - p0 - 16 * s2 - 4 * g;  // positions 0..3 and 8..11 from here are this lane's
-                            half8_t seen_v = vf.whole;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if ((e & 3) + 8 * (e >> 2) >= end) seen_v[e] = static_cast<half_t>(0.0f);
-                            floatx16 with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, ph, o[dt], 0, 0, 0);
-                            if constexpr (kLo) with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
-                            if (my_tok == t0 + token) o[dt] = with;
-                        }
-                        continue;
+                        for (int e = 0; e < 8; ++e)
+                            if ((e & 3) + 8 * (e >> 2) >= end) seen_v[e] = static_cast<half_t>(0.0f);
+                        floatx16 with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, ph, o[dt], 0, 0, 0);
+                        if constexpr (kLo) with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
+                        if (my_tok == t0 + token) o[dt] = with;
                     }
                 }
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, ph, o[dt], 0, 0, 0);
-                if constexpr (kLo) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf.whole, pl, o[dt], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int dt = 0; dt < kDTiles; ++dt) {
+                    const half8_t v = values_of(s2, dt);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[dt], 0, 0, 0);
+                    if constexpr (kLo) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[dt], 0, 0, 0);
+                }
             }
         }
         lsum += step_sum;
@@ -325,9 +358,15 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if constexpr (kR > 1) __syncthreads();
         if (turn + 1 < turns) request(turn + 1);
-        const char* stage = stages + (turn % S::kStages) * S::kStageBytes;
-        if (p0 + kStep <= t0 + 1) walk(std::false_type{}, p0, stage);  // (uniform)
-        else if (p0 < wave_limit) walk(std::true_type{}, p0, stage);
+        const char* keys = stages + (turn % S::kStages) * S::kStageBytes;
+        const char* values = keys + S::kHalfBytes;
+        if (p0 + kStep <= t0 + 1) {  // (uniform)
+            walk(std::false_type{}, std::integral_constant<int, kTiles>{}, p0, keys, values);
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < kTiles && p0 + 32 * t < wave_limit; ++t)
+                walk(std::true_type{}, std::integral_constant<int, 1>{}, p0 + 32 * t, keys + t * 32 * kRowBytes, values + t * 32 * kRowBytes);
+        }
     }
     lsum = halves_sum(lsum);
     T* out_row = static_cast<T*>(job.out) + static_cast<size_t>(first_row + tok_c) * job.out_stride + (kvh * job.shared + my_head) * kHs + 4 * g;
@@ -418,11 +457,18 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
     return LPP_OK;
 }
 
+// Which shape: the fewer tiles of 32 rows there are for each compute unit, the more wavefronts share a walk.  us, one prompt, 1 x 4 / 2 x 2 /
+// 4 x 1, 32 heads of 64 on 8, fp32: 256 rows (one tile a compute unit) 6.3 / 7.9 / 10.3; 512 9.3 / 11.7 / 14.8; 700 15.9 / 15.1 / 17.2; 1024 21.6 /
+// 20.7 / 24.1; 1500 38.6 / 33.3 / 34.5; 2048 59 / 56 / 49; 6000 - / 338 / 284.  32 heads of 128, binary16: 256 6.9 / 8.4 / 10.8; 400
+// 12.2 / 11.0 / 13.2; 1024 34 / 22 / 27; 1500 59 / 36 / 39; 2048 95 / 59 / 55; 6000 - / 381 / 321.  Steps of 4 x 1: 128 positions (heads of 64;
+// 64: 302 us at 6000 rows) or 64 (heads of 128; 32: 350).  (8 x 1: 326 and 331; the products of the next step formed between this
+// one's weights, a third stage, or other priorities for the products: no faster.)
 template <typename T, int kHs>
 lpp_status launch(const PromptJob& job, int n_seqs) {
     const long long tiles = (static_cast<long long>(job.n_tokens) * job.shared + 31) / 32 * job.n_kv_heads;  // of 32 rows
-    if (tiles <= 2ll * compute_units()) return launch_as<T, kHs, 1, 4, 32>(job, n_seqs);
-    return launch_as<T, kHs, 4, 1, 64>(job, n_seqs);
+    if (tiles <= (kHs == 64 ? 2ll : 1ll) * compute_units()) return launch_as<T, kHs, 1, 4, 32>(job, n_seqs);
+    if (tiles <= 6ll * compute_units()) return launch_as<T, kHs, 2, 2, 32>(job, n_seqs);
+    return launch_as<T, kHs, 4, 1, kHs == 64 ? 128 : 64>(job, n_seqs);
 }
 
 }  // namespace
