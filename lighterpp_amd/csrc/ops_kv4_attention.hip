@@ -24,16 +24,21 @@ struct AttendJob {
     float* mass;
     float2* stats;     // [sequence][KV head][tile][range][16]: maximum (in powers of two) and sum of a range
     float* partials;   // [sequence][KV head][tile][range][16][head_size]
-    int n_q, n_kv_heads, shared, seq_len, splits, least, tiles;
+    unsigned heads;  // n_seqs times n_kv_heads
+    int n_seqs, n_q, n_kv_heads, shared, seq_len, splits, least, tiles;
+    float per_workgroup;  // KV heads times tiles over the workgroups there should be
     unsigned per_shared;  // 65536 / shared, rounded up: column * per_shared >> 16 is column / shared for columns below 16
     // (a start outside -n_q .. seq_len says no more than the ends of that)
     __device__ __forceinline__ int start_of(int s) const { return min(max(starts[s], -n_q), seq_len); }
     __device__ __forceinline__ int end_of(int start, int row) const { return min(max(start + row + 1, 0), seq_len); }
     __device__ __forceinline__ int tokens() const { return static_cast<int>(kRows * per_shared >> 16); }  // of a tile
-    // How many of `positions` a range has: whole steps of four wavefronts, `least` at least.
-    __device__ __forceinline__ int range_of(int positions) const {
-        const int even = (positions + splits - 1) / splits;
-        return max(least, (even + 4 * kStep - 1) / (4 * kStep) * (4 * kStep));
+    // How many shares a sequence's `positions` are cut into: of all sequences' positions, as many to each as gives `workgroups` of them in all,
+    // but no fewer than `least`.  (All lanes call it and read the sequences' starts, 64 at a time; the same sum in every workgroup.)
+    __device__ __forceinline__ int shares_of(int positions) const {
+        float all = 0.0f;
+        for (int s0 = 0; s0 < n_seqs; s0 += kWave) all += wave_sum(s0 + lane_id() < n_seqs ? static_cast<float>(end_of(start_of(s0 + lane_id()), n_q - 1)) : 0.0f);
+        const int each = max(least, static_cast<int>(fminf(all * per_workgroup, 1e9f)));
+        return max(min((positions + each - 1) / each, splits), 1);
     }
 };
 
@@ -44,32 +49,43 @@ __device__ __forceinline__ float rows_max(float v) {
     const auto halves = __builtin_amdgcn_permlane32_swap(m, m, false, false);
     return fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
 }
-// A lane's part of 16 rows of codes: of position lane % 16, the kHs / 4 values from kHs / 4 * (lane / 16) on.
+// A lane's part of 16 rows of codes: of position lane % 16, the kHs / 4 values from kHs / 4 * (lane / 16) on, and their scale and lowest
+// value.
 template <int kHs>
 struct Piece {
     static constexpr int kWords = kHs / 32;
     uint32_t codes[kWords], pair;
     // (a head's rows are within 2^31 bytes: a uniform base and an offset of 32 bits)
-    __device__ __forceinline__ void load(const uint32_t* codes_of_head, const uint32_t* scales_of_head, int pos, int part) {
-        const uint32_t row = static_cast<uint32_t>(pos);
-        const char* from = reinterpret_cast<const char*>(codes_of_head) + (row * (kHs / 2) + static_cast<uint32_t>(part) * (kWords * 4));
-        if constexpr (kWords == 4) {
-            const uintx4 all = load16(from);
+    __device__ __forceinline__ void load(const uint32_t* codes_of_head, int pos, int part) {
+        const char* from = reinterpret_cast<const char*>(codes_of_head) + (static_cast<uint32_t>(pos) * (kHs / 2) + static_cast<uint32_t>(part) * (kWords * 4));
+        typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
+        const Words all = __builtin_nontemporal_load(reinterpret_cast<const Words*>(from));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) codes[i] = all[i];
-        } else {
-            const uint2 all = *reinterpret_cast<const uint2*>(from);
-            codes[0] = all.x;
-            codes[1] = all.y;
-        }
-        pair = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(scales_of_head) +
-                                                  (row * (kHs / 8) + static_cast<uint32_t>(part * kWords / 4) * 4));
+        for (int i = 0; i < kWords; ++i) codes[i] = all[i];
     }
     __device__ __forceinline__ half8_t values(const Kv4Reader& read, int i) const { return read(codes[i], pair); }
     // Whether a value may be infinite or NaN.
     __device__ __forceinline__ bool may_be_nonfinite() const {
         const half2_t both = __builtin_bit_cast(half2_t, pair);
         return !(fmaf(15.0f, fabsf(static_cast<float>(both[0])), fabsf(static_cast<float>(both[1]))) < 65504.0f);
+    }
+};
+
+// The scales of 64 rows (32 of K and 32 of V, or 64 of K): a lane requests a row's and a wavefront all of them at once; through its own LDS they get
+// to the lanes that have the codes.  (Requested by those lanes, four bytes each, they are four requests in eight, and a fifth of the bytes
+// took a third of the time: a batch of 32 sequences of up to 8000 positions, heads of 128, 69 us for reading alone, 47 so.)
+template <int kHs>
+struct ScaleRows {
+    static constexpr int kWords = kHs / kKv4Group, kRowBytes = 4 * kWords, kLdsBytes = 64 * kRowBytes;
+    typedef uint32_t Row __attribute__((ext_vector_type(kWords)));
+    Row row;
+    __device__ __forceinline__ void load(const uint32_t* scales_of_head, int pos) {
+        row = __builtin_nontemporal_load(reinterpret_cast<const Row*>(reinterpret_cast<const char*>(scales_of_head) + static_cast<uint32_t>(pos) * kRowBytes));
+    }
+    __device__ __forceinline__ void put(char* lds) const { *reinterpret_cast<Row*>(lds + lane_id() * kRowBytes) = row; }
+    // scale and lowest value of row `row` for the values of a Piece
+    static __device__ __forceinline__ uint32_t get(const char* lds, int row, int part) {
+        return *reinterpret_cast<const uint32_t*>(lds + row * kRowBytes + part * kWords / 4 * 4);
     }
 };
 
@@ -154,19 +170,24 @@ template <int kHs, int kWaves>
 __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kernel(AttendJob job) {
     constexpr int kDTiles = kHs / 16, kWords = kHs / 32, kRowBytes = 2 * kHs, kThreads = kWave * kWaves;
     constexpr int kPad = kHs + 4, kPart = kRows * kPad + 2 * kRows;  // floats a wavefront leaves for the merge
-    constexpr int kWaveBytes = kPart * 4;
-    static_assert(kWaveBytes >= kStep * kRowBytes, "V rows of a step");
+    constexpr int kWaveBytes = kPart * 4 + ScaleRows<kHs>::kLdsBytes;
+    static_assert(kPart * 4 >= kStep * kRowBytes && kWaveBytes % 16 == 0, "V rows of a step");
     extern __shared__ __align__(16) char lds[];
     const int lane = lane_id(), wave = wave_index(), column = lane & 15, part = lane >> 4;
-    const int split = static_cast<int>(blockIdx.x) % job.splits, tile = static_cast<int>(blockIdx.x) / job.splits, kvh = blockIdx.y, s = blockIdx.z;
+    // (Heads of sequences first, then a head's tiles, then the shares: whatever number of the shares there are, the workgroups that have one are
+    // dealt out evenly over the dies, and the tiles of a head, which read the same rows, go to the same die where the heads
+    // are a multiple of its number.)
+    const int head = static_cast<int>(blockIdx.x % job.heads), rest = static_cast<int>(blockIdx.x / job.heads);
+    const int kvh = head % job.n_kv_heads, s = head / job.n_kv_heads, tile = rest % job.tiles, split = rest / job.tiles;
     const int tokens = job.tokens(), start = job.start_of(s);
     const int all_end = job.end_of(start, job.n_q - 1);
-    const int range = job.range_of(all_end);
-    const int begin = split * range;
-    if (begin >= all_end && split > 0) return;
-    const int tile_end = job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1);
-    const int end = min(begin + range, tile_end);  // (at or before `begin`: the tile's rows attend to nothing here)
-    const bool only = range >= all_end;            // (uniform over the sequence: no merge)
+    const int shares = job.shares_of(all_end);
+    if (split >= shares) return;
+    const int end = job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1);  // the tile's last row attends to [0, end)
+    const bool only = shares == 1;                                               // (uniform over the sequence: no merge)
+    // A workgroup's steps are one for each of its wavefronts in every round of all shares' workgroups: what they read at a time is one
+    // stretch of the head's rows.
+    const int first = (split * kWaves + wave) * kStep, stride = shares * kWaves * kStep;
     const Column mine(job, tile, column);
     const int my_end = job.end_of(start, mine.token), first_end = job.end_of(start, tile * tokens);
     const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
@@ -181,10 +202,14 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     Piece<kHs> k[2], v[2];
     auto request = [&](Piece<kHs>(&to)[2], int which, int p0) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) to[t].load(codes[which], scales[which], min(p0 + 16 * t + column, end - 1), part);
+        for (int t = 0; t < 2; ++t) to[t].load(codes[which], min(p0 + 16 * t + column, end - 1), part);
     };
-    const int first = begin + wave * kStep;
+    ScaleRows<kHs> pairs;
+    char* pairs_lds = lds + wave * kWaveBytes + kPart * 4;
+    const uint32_t* my_scales = lane < 32 ? scales[0] : scales[1];
+    auto request_pairs = [&](int p0) { pairs.load(my_scales, min(p0 + (lane & 31), end - 1)); };
     if (first < end) {
+        request_pairs(first);
         request(k, 0, first);
         request(v, 1, first);
     }
@@ -215,24 +240,31 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         for (int i = 0; i < kWords; ++i) v_to[i] = column * kRowBytes + 16 * ((kWords * part + i) ^ swizzle(column));
     }
 
-    for (int p0 = first; p0 < end; p0 += kStep * kWaves) {
-        const bool more = p0 + kStep * kWaves < end;  // (uniform)
+    for (int p0 = first; p0 < end; p0 += stride) {
+        const bool more = p0 + stride < end;         // (uniform)
         const bool partly = p0 + kStep > first_end;   // (uniform) some row does not attend to the whole step
+        pairs.put(pairs_lds);
+        if (more) request_pairs(p0 + stride);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            k[t].pair = ScaleRows<kHs>::get(pairs_lds, 16 * t + column, part);
+            v[t].pair = ScaleRows<kHs>::get(pairs_lds, 32 + 16 * t + column, part);
+        }
         floatx4 st[2];
         q.template scores<2>(read, k, st);
-        if (more) request(k, 0, p0 + kStep * kWaves);
+        if (more) request(k, 0, p0 + stride);
         // V rows behind the tile's last position are zero: a weight of zero does not keep an infinity or NaN out.
         if (partly) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                if (p0 + 16 * t + column >= tile_end) v[t].pair = 0u;
+                if (p0 + 16 * t + column >= end) v[t].pair = 0u;
         }
         const bool odd = __builtin_amdgcn_ballot_w64(v[0].may_be_nonfinite() || v[1].may_be_nonfinite()) != 0ull;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < kWords; ++i) *reinterpret_cast<half8_t*>(values + v_to[i] + 16 * t * kRowBytes) = v[t].values(read, i);
-        if (more) request(v, 1, p0 + kStep * kWaves);
+        if (more) request(v, 1, p0 + stride);
         if (partly) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -315,10 +347,11 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
 
     // The wavefronts meet in LDS, each thread adding four values of a row in the order of the wavefronts.  Those that had no step have left
     // nothing and are not read.
-    const int steps = max((end - begin + kStep - 1) / kStep, 0), parts = max(min(steps, kWaves), 1);
+    const int parts = min(max((end - split * kWaves * kStep + kStep - 1) / kStep, 1), kWaves);
+    constexpr int kPartStep = kWaveBytes / 4;
     float* all = reinterpret_cast<float*>(lds);
     if (wave < parts) {
-        float* my_part = all + wave * kPart;
+        float* my_part = all + wave * kPartStep;
 #pragma unroll
         for (int dt = 0; dt < kDTiles; ++dt) *reinterpret_cast<floatx4*>(my_part + column * kPad + 16 * dt + 4 * part) = o[dt];
         if (part == 0) {
@@ -333,14 +366,14 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     for (int i = threadIdx.x; i < used * kFours; i += kThreads) {
         const int row = i / kFours, four = i % kFours;
         float all_top = -INFINITY, total = 0.0f;
-        for (int w = 0; w < parts; ++w) all_top = fmaxf(all_top, all[w * kPart + kRows * kPad + row]);
+        for (int w = 0; w < parts; ++w) all_top = fmaxf(all_top, all[w * kPartStep + kRows * kPad + row]);
         const float reference = all_top == -INFINITY ? 0.0f : all_top;  // (nothing seen, or no score was a number)
         floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int w = 0; w < parts; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(all[w * kPart + kRows * kPad + row] - reference);
-            total = fmaf(all[w * kPart + kRows * kPad + kRows + row], weight, total);
-            const floatx4 a = *reinterpret_cast<const floatx4*>(all + w * kPart + row * kPad + 4 * four);
+            const float weight = __builtin_amdgcn_exp2f(all[w * kPartStep + kRows * kPad + row] - reference);
+            total = fmaf(all[w * kPartStep + kRows * kPad + kRows + row], weight, total);
+            const floatx4 a = *reinterpret_cast<const floatx4*>(all + w * kPartStep + row * kPad + 4 * four);
 #pragma unroll
             for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[u], weight, sum[u]);
         }
@@ -358,25 +391,26 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     }
 }
 
-// What is left once every range has been walked: blocks before `merges` (where there are ranges to merge) merge a row each, the others add up
-// the weights of kMassPositions positions each.
+// What is left once every share has been walked: blocks before `merges` (where there are shares to merge) merge a row each, the others add up
+// the weights of the positions, kPieces * 64 at a time.
 constexpr int kFinishWaves = 4, kFinishThreads = kWave * kFinishWaves;
-constexpr int kMassPositions = 256;
 
-template <int kHs>
-__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges) {
+template <int kHs, int kPieces>
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges, int mass_rounds) {
     constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours;
     __shared__ float weights[kMaxSplits];
     __shared__ __align__(16) float partial[kSlices][kHs];
     __shared__ float tops[kRows], inverses[kRows];
+    __shared__ __align__(16) char scale_lds[kFinishWaves][ScaleRows<kHs>::kLdsBytes];
     __shared__ __align__(16) char q_lds[Queries<kHs>::kLdsBytes > 0 ? Queries<kHs>::kLdsBytes : 16];
     const int lane = lane_id(), wave = wave_index(), column = lane & 15, part = lane >> 4;
-    const int kvh = blockIdx.y, s = blockIdx.z, start = job.start_of(s), tokens = job.tokens();
+    const int head = static_cast<int>(blockIdx.x % job.heads), block = static_cast<int>(blockIdx.x / job.heads);
+    const int kvh = head % job.n_kv_heads, s = head / job.n_kv_heads, start = job.start_of(s), tokens = job.tokens();
     const int all_end = job.end_of(start, job.n_q - 1);
-    const int range = job.range_of(all_end), active = max((all_end + range - 1) / range, 1);
-    if (static_cast<int>(blockIdx.x) < merges) {
+    const int active = job.shares_of(all_end);
+    if (block < merges) {
         if (active == 1) return;
-        const int tile = static_cast<int>(blockIdx.x) / kRows, row = static_cast<int>(blockIdx.x) % kRows;
+        const int tile = block / kRows, row = block % kRows;
         const Column its(job, tile, row);
         if (!its.valid) return;
         const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
@@ -386,6 +420,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         floatx4 a[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
+            if (kSlices * i >= active) break;  // (uniform)
             const int at = min(slice + kSlices * i, active - 1);
             a[i] = *reinterpret_cast<const floatx4*>(job.partials + ((slot + at) * kRows + row) * kHs + 4 * four);
         }
@@ -399,6 +434,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
+            if (kSlices * i >= active) break;
             const int at = slice + kSlices * i;
             const float w = weights[at];
             if (at < active && w >= 0.0f)
@@ -415,97 +451,130 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         }
         return;
     }
-    const int p_first = (static_cast<int>(blockIdx.x) - merges) * kMassPositions;
-    if (p_first >= all_end) return;
+    // (rounds of kRound positions, one for each block of the sequence and head in turn)
+    constexpr int kOfWave = 16 * kPieces, kRound = kOfWave * kFinishWaves;
+    const int blocks = (all_end + kRound * mass_rounds - 1) / (kRound * mass_rounds);
+    const int p_first = (block - merges) * kRound;
+    if (block - merges >= blocks) return;
     const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
     const uint32_t* codes = job.cache.codes[0] + head_rows * (kHs / 8);
     const uint32_t* scales = job.cache.scales[0] + head_rows * (kHs / kKv4Group);
     float* mass = job.mass + head_rows;
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
-    constexpr int kPieces = kMassPositions / (16 * kFinishWaves);
-    Piece<kHs> k[kPieces];
-    floatx4 sum[kPieces];  // of this lane's column, over the tiles
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-        k[i].load(codes, scales, min(p_first + 16 * (wave + kFinishWaves * i) + column, all_end - 1), part);
-        sum[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    // (a lane adds the weights of one position a piece: position 4 part + column, for columns below four)
-    float before[kPieces];
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-        const int p = p_first + 16 * (wave + kFinishWaves * i) + 4 * part + column;
-        before[i] = column < 4 && p < all_end ? mass[p] : 0.0f;
-    }
+    const int columns = min(tokens, job.n_q) * job.shared;
     const Kv4Reader read;
-    for (int tile = 0; tile < job.tiles; ++tile) {
-        if (job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1) <= p_first) continue;  // (uniform)
-        const Column mine(job, tile, column);
-        const int my_end = mine.valid ? job.end_of(start, mine.token) : 0;
-        if (tile > 0) __syncthreads();  // (the tile before is done with what LDS holds)
-        Queries<kHs> q;
-        q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds, wave, kFinishWaves);
-        // (maximum, 1 / sum) of the tile's rows: 16 threads to a row
-        {
-            const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
-            const int row = threadIdx.x / 16, at = threadIdx.x % 16;
-            const bool live = row < min(tokens, job.n_q - tile * tokens) * job.shared;
-            float2 st[kMaxSplits / 16];
-            float top = -INFINITY, total = 0.0f;
+    const int last = all_end;
+    // (a wavefront has kOfWave neighbouring positions of a round)
+    Piece<kHs> k[kPieces], next[kPieces];
+    ScaleRows<kHs> pairs;
+    char* pairs_lds = scale_lds[wave];
+    auto request = [&](int base) {
+        pairs.load(scales, min(base + kOfWave * wave + (lane & (kOfWave - 1)), last - 1));
 #pragma unroll
-            for (int i = 0; i < kMaxSplits / 16; ++i) {
-                st[i] = make_float2(-INFINITY, 0.0f);
-                if (live && at + 16 * i < active) st[i] = job.stats[(slot + at + 16 * i) * kRows + row];
-                top = fmaxf(top, st[i].x);
+        for (int i = 0; i < kPieces; ++i) next[i].load(codes, min(base + kOfWave * wave + 16 * i + column, last - 1), part);
+    };
+    request(p_first);
+    Queries<kHs> q;
+    float top = 0.0f, inverse = 0.0f;
+    int loaded = -1;  // the tile that `q`, `top` and `inverse` are of
+    for (int base = p_first; base < last; base += blocks * kRound) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) k[i] = next[i];
+        pairs.put(pairs_lds);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) k[i].pair = ScaleRows<kHs>::get(pairs_lds, 16 * i + column, part);
+        if (base + blocks * kRound < last) request(base + blocks * kRound);
+        floatx4 sum[kPieces];  // of this lane's column, over the tiles
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) sum[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        // (a lane adds the weights of one position a piece: position 4 part + column, for columns below four)
+        float before[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int p = base + kOfWave * wave + 16 * i + 4 * part + column;
+            before[i] = column < 4 && p < last ? mass[p] : 0.0f;
+        }
+        for (int tile = 0; tile < job.tiles; ++tile) {
+            if (job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1) <= base) continue;  // (uniform)
+            const Column mine(job, tile, column);
+            const int my_end = mine.valid ? job.end_of(start, mine.token) : 0;
+            if (loaded != tile) {
+                if (loaded >= 0) __syncthreads();  // (the tile before is done with what LDS holds)
+                loaded = tile;
+                q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds, wave, kFinishWaves);
+                // (maximum, 1 / sum) of the tile's rows: 16 threads to a row
+                const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
+                const int row = threadIdx.x / 16, at = threadIdx.x % 16;
+                const bool live = row < min(tokens, job.n_q - tile * tokens) * job.shared;
+                float2 st[kMaxSplits / 16];
+                float highest = -INFINITY, total = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kMaxSplits / 16; ++i) {
+                    st[i] = make_float2(-INFINITY, 0.0f);
+                    if (live && at + 16 * i < active) st[i] = job.stats[(slot + at + 16 * i) * kRows + row];
+                    highest = fmaxf(highest, st[i].x);
+                }
+                highest = fmaxf(highest, dpp_move<kDppXor1>(highest));
+                highest = fmaxf(highest, dpp_move<kDppXor2>(highest));
+                highest = fmaxf(highest, dpp_move<kDppHalfMirror>(highest));
+                highest = fmaxf(highest, dpp_move<kDppMirror>(highest));
+                if (highest == -INFINITY) highest = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kMaxSplits / 16; ++i) total = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - highest), total);
+                total = row16_sum(total);
+                if (at == 0) {
+                    tops[row] = highest;
+                    inverses[row] = 1.0f / total;
+                }
+                __syncthreads();
+                top = tops[column];
+                inverse = inverses[column];
             }
-            top = fmaxf(top, dpp_move<kDppXor1>(top));
-            top = fmaxf(top, dpp_move<kDppXor2>(top));
-            top = fmaxf(top, dpp_move<kDppHalfMirror>(top));
-            top = fmaxf(top, dpp_move<kDppMirror>(top));
-            if (top == -INFINITY) top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kMaxSplits / 16; ++i) total = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - top), total);
-            total = row16_sum(total);
-            if (at == 0) {
-                tops[row] = top;
-                inverses[row] = 1.0f / total;
+            for (int i = 0; i < kPieces; i += 2) {
+                floatx4 st[2];
+                q.template scores<2>(read, k + i, st);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -top)) * inverse;
+                        sum[i + t][e] += base + kOfWave * wave + 16 * (i + t) + 4 * part + e < my_end ? w : 0.0f;
+                    }
             }
         }
-        __syncthreads();
-        const float top = tops[column], inverse = inverses[column];
 #pragma unroll
-        for (int i = 0; i < kPieces; i += 2) {
-            floatx4 st[2];
-            q.template scores<2>(read, k + i, st);
+        for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int e = 0; e < 4; ++e) {
+                sum[i][e] += dpp_move<kDppXor1>(sum[i][e]);
+                sum[i][e] += dpp_move<kDppXor2>(sum[i][e]);
+            }
+            if (columns > 4) {  // (uniform; columns that no row has have added nothing)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -top)) * inverse;
-                    sum[i + t][e] += p_first + 16 * (wave + kFinishWaves * (i + t)) + 4 * part + e < my_end ? w : 0.0f;
+                    sum[i][e] += dpp_move<kDppHalfMirror>(sum[i][e]);
+                    sum[i][e] += dpp_move<kDppMirror>(sum[i][e]);
                 }
+            }
+            const int p = base + kOfWave * wave + 16 * i + 4 * part + column;
+            if (column < 4 && p < last) mass[p] = before[i] + (column == 0 ? sum[i][0] : column == 1 ? sum[i][1] : column == 2 ? sum[i][2] : sum[i][3]);
         }
-    }
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[i][e] = row16_sum(sum[i][e]);
-        const int p = p_first + 16 * (wave + kFinishWaves * i) + 4 * part + column;
-        if (column < 4 && p < all_end) mass[p] = before[i] + (column == 0 ? sum[i][0] : column == 1 ? sum[i][1] : column == 2 ? sum[i][2] : sum[i][3]);
     }
 }
 
 int tiles_of(int n_q, int shared) { return (n_q + kRows / shared - 1) / (kRows / shared); }
 
-// Ranges a sequence's positions are cut into, the least positions of one, and the wavefronts to one.
+// Shares a sequence's positions are cut into at most, the least positions of one, the wavefronts to one, and how many of them there should be.
 struct Split {
-    int splits, least, waves;
+    int splits, least, waves, workgroups;
 };
 Split split_of(const lpp_kv4_shape& shape, int tiles) {
     const long long heads = static_cast<long long>(shape.n_seqs) * shape.n_kv_heads * tiles;
     Split s;
     s.waves = heads * 4 > compute_units() ? 4 : shape.head_size == 64 ? 16 : 8;
-    s.least = heads >= 2ll * compute_units() ? 2048 : heads * 4 > compute_units() ? 1024 : 512;
+    s.least = 512;
+    s.workgroups = compute_units() * (shape.head_size == 64 ? 16 : 12) / s.waves;
     const int most = (shape.seq_len + s.least - 1) / s.least;
     s.splits = most < kMaxSplits ? most : kMaxSplits;
     return s;
@@ -513,7 +582,7 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
 
 template <int kHs, int kWaves>
 lpp_status launch_attend(const AttendJob& job, dim3 grid) {
-    constexpr int kLds = kWaves * (kRows * (kHs + 4) + 2 * kRows) * 4 + Queries<kHs>::kLdsBytes;
+    constexpr int kLds = kWaves * ((kRows * (kHs + 4) + 2 * kRows) * 4 + ScaleRows<kHs>::kLdsBytes) + Queries<kHs>::kLdsBytes;
     const auto kernel = &attend_kernel<kHs, kWaves>;
     if constexpr (kLds > 64 * 1024) {  // told to the runtime once per device
         static bool sized[64] = {};
@@ -575,6 +644,8 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     job.cache = kv4_layer(d_cache, *shape, layer);
     job.starts = d_starts;
     job.mass = d_mass != nullptr ? d_mass + kv4_layer_rows(*shape) * layer : nullptr;
+    job.heads = static_cast<unsigned>(shape->n_seqs) * shape->n_kv_heads;
+    job.n_seqs = shape->n_seqs;
     job.n_q = n_q;
     job.n_kv_heads = shape->n_kv_heads;
     job.shared = n_heads / shape->n_kv_heads;
@@ -583,23 +654,29 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     const Split split = split_of(*shape, job.tiles);
     job.splits = split.splits;
     job.least = split.least;
+    job.per_workgroup = static_cast<float>(shape->n_kv_heads) * job.tiles / split.workgroups;
     job.per_shared = (65536u + job.shared - 1) / job.shared;
     const size_t slots = static_cast<size_t>(shape->n_seqs) * shape->n_kv_heads * job.tiles * job.splits;
     job.stats = static_cast<float2*>(d_workspace);
     job.partials = reinterpret_cast<float*>(job.stats + slots * kRows);
-    const dim3 grid(static_cast<unsigned>(job.splits) * job.tiles, shape->n_kv_heads, shape->n_seqs);
+    const long long groups = static_cast<long long>(job.heads) * job.tiles * job.splits;
+    LPP_REQUIRE(groups * dev::kWave * split.waves < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads and %d rows are too many for a launch", job.heads, n_q);
+    const dim3 grid(static_cast<unsigned>(groups));
     if (shape->head_size == 64)
         LPP_TRY(split.waves == 16 ? (launch_attend<64, 16>(job, grid)) : (launch_attend<64, 4>(job, grid)));
     else
         LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
     const int merges = job.splits > 1 ? job.tiles * kRows : 0;
-    const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + kMassPositions - 1) / kMassPositions : 0);
+    // The account: several tiles (more than 16 rows) take 256 positions at a time, K once for all of them, and one such round to a block: what
+    // counts is how often a tile's queries are read.  One tile: 128 at a time, four wavefronts to a SIMD, and 8 rounds.
+    const int round = job.tiles > 1 ? 256 : 128, mass_rounds = job.tiles > 1 ? 1 : 8;
+    const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + round * mass_rounds - 1) / (round * mass_rounds) : 0);
     if (blocks > 0) {
-        const dim3 rest(blocks, shape->n_kv_heads, shape->n_seqs);
-        if (shape->head_size == 64)
-            hipLaunchKernelGGL(finish_kernel<64>, rest, dim3(kFinishThreads), 0, stream(), job, merges);
-        else
-            hipLaunchKernelGGL(finish_kernel<128>, rest, dim3(kFinishThreads), 0, stream(), job, merges);
+        LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch",
+                    job.heads, shape->seq_len);
+        const auto kernel = shape->head_size == 64 ? (job.tiles > 1 ? &finish_kernel<64, 4> : &finish_kernel<64, 2>)
+                                                   : (job.tiles > 1 ? &finish_kernel<128, 4> : &finish_kernel<128, 2>);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, merges, mass_rounds);
         LPP_CHECK_LAUNCH("finish_kernel");
     }
     return LPP_OK;
