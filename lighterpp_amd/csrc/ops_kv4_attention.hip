@@ -345,8 +345,8 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     lsum = rows_sum(lsum);
     if (!seen) top = -INFINITY;
 
-    // The wavefronts meet in LDS, each thread adding four values of a row in the order of the wavefronts.  Those that had no step have left
-    // nothing and are not read.
+    // The wavefronts meet in LDS: four neighbouring lanes add four values of a row, each a quarter of the wavefronts in their order.  Those that
+    // had no step have left nothing and are not read.
     const int parts = min(max((end - split * kWaves * kStep + kStep - 1) / kStep, 1), kWaves);
     constexpr int kPartStep = kWaveBytes / 4;
     float* all = reinterpret_cast<float*>(lds);
@@ -363,20 +363,41 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits + split;
     constexpr int kFours = kHs / 4;
     const int used = min(tokens, job.n_q - tile * tokens) * job.shared;  // rows there are
-    for (int i = threadIdx.x; i < used * kFours; i += kThreads) {
-        const int row = i / kFours, four = i % kFours;
-        float all_top = -INFINITY, total = 0.0f;
-        for (int w = 0; w < parts; ++w) all_top = fmaxf(all_top, all[w * kPartStep + kRows * kPad + row]);
+    const int quarter = lane & 3;
+    // (whole wavefronts go round: the lanes of a quarter are all here)
+    for (int i = static_cast<int>(threadIdx.x) / 4; i < (used * kFours + 15) / 16 * 16; i += kThreads / 4) {
+        const bool there = i < used * kFours;
+        const int row = there ? i / kFours : 0, four = i % kFours;
+        constexpr int kMine = kWaves / 4;
+        float weight[kMine], all_top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int w = quarter * kMine + j;
+            weight[j] = w < parts ? all[w * kPartStep + kRows * kPad + row] : -INFINITY;
+            all_top = fmaxf(all_top, weight[j]);
+        }
+        all_top = fmaxf(all_top, dpp_move<kDppXor1>(all_top));
+        all_top = fmaxf(all_top, dpp_move<kDppXor2>(all_top));
         const float reference = all_top == -INFINITY ? 0.0f : all_top;  // (nothing seen, or no score was a number)
         floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int w = 0; w < parts; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(all[w * kPartStep + kRows * kPad + row] - reference);
-            total = fmaf(all[w * kPartStep + kRows * kPad + kRows + row], weight, total);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int w = quarter * kMine + j;
+            if (w >= parts) break;
+            weight[j] = __builtin_amdgcn_exp2f(weight[j] - reference);
+            total = fmaf(all[w * kPartStep + kRows * kPad + kRows + row], weight[j], total);
             const floatx4 a = *reinterpret_cast<const floatx4*>(all + w * kPartStep + row * kPad + 4 * four);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[u], weight, sum[u]);
+            for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[u], weight[j], sum[u]);
         }
+        total += dpp_move<kDppXor1>(total);
+        total += dpp_move<kDppXor2>(total);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            sum[u] += dpp_move<kDppXor1>(sum[u]);
+            sum[u] += dpp_move<kDppXor2>(sum[u]);
+        }
+        if (!there || quarter != 0) continue;
         if (only) {
             const Column its(job, tile, row);
             const bool any = job.end_of(start, its.token) > 0;
@@ -565,16 +586,19 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
 
 int tiles_of(int n_q, int shared) { return (n_q + kRows / shared - 1) / (kRows / shared); }
 
-// Shares a sequence's positions are cut into at most, the least positions of one, the wavefronts to one, and how many of them there should be.
+// Shares a sequence's positions are cut into at most, the least positions of one, the wavefronts to one, and how many of them run at once.
+// Few heads: 8 wavefronts to a share, for half the steps of each (one sequence of 8 KV heads of 64, us at 500 / 1000 / 8000 positions: 6.4 / 9.3 / 9.4,
+// 6.8 / 9.7 / 9.8 with 4 and 6.7 / 9.6 / 9.8 with 16; of 128: 8.2 / 10.9 / 11.4, 9.4 / 12.2 / 12.6 with 4).  512 positions at least: 256
+// or 1024 give one sequence of 16001 10.1 or 9.7 us for 8.0, and more or fewer shares to merge.
 struct Split {
     int splits, least, waves, workgroups;
 };
 Split split_of(const lpp_kv4_shape& shape, int tiles) {
     const long long heads = static_cast<long long>(shape.n_seqs) * shape.n_kv_heads * tiles;
     Split s;
-    s.waves = heads * 4 > compute_units() ? 4 : shape.head_size == 64 ? 16 : 8;
+    s.waves = heads * 4 > compute_units() ? 4 : 8;
     s.least = 512;
-    s.workgroups = compute_units() * (shape.head_size == 64 ? 16 : 12) / s.waves;
+    s.workgroups = compute_units() * (shape.head_size == 64 ? 16 / s.waves : s.waves == 8 ? 1 : 3);  // (by registers, and LDS for the heads of 128)
     const int most = (shape.seq_len + s.least - 1) / s.least;
     s.splits = most < kMaxSplits ? most : kMaxSplits;
     return s;
@@ -663,13 +687,16 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     LPP_REQUIRE(groups * dev::kWave * split.waves < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads and %d rows are too many for a launch", job.heads, n_q);
     const dim3 grid(static_cast<unsigned>(groups));
     if (shape->head_size == 64)
-        LPP_TRY(split.waves == 16 ? (launch_attend<64, 16>(job, grid)) : (launch_attend<64, 4>(job, grid)));
+        LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
     else
         LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
     const int merges = job.splits > 1 ? job.tiles * kRows : 0;
     // The account: several tiles (more than 16 rows) take 256 positions at a time, K once for all of them, and one such round to a block: what
-    // counts is how often a tile's queries are read.  One tile: 128 at a time, four wavefronts to a SIMD, and 8 rounds.
-    const int round = job.tiles > 1 ? 256 : 128, mass_rounds = job.tiles > 1 ? 1 : 8;
+    // counts is how often a tile's queries are read.  One tile: 128 at a time, and as many rounds to a block, up to 8, as leave three blocks
+    // to a compute unit.
+    const int round = job.tiles > 1 ? 256 : 128;
+    const long long rounds = (static_cast<long long>(shape->seq_len) + round - 1) / round * job.heads / (3 * compute_units());
+    const int mass_rounds = job.tiles > 1 || rounds < 1 ? 1 : rounds < 8 ? static_cast<int>(rounds) : 8;
     const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + round * mass_rounds - 1) / (round * mass_rounds) : 0);
     if (blocks > 0) {
         LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch",
