@@ -413,17 +413,19 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
 }
 
 // What is left once every share has been walked: blocks before `merges` (where there are shares to merge) merge a row each, the others add up
-// the weights of the positions, kPieces * 64 at a time.
+// the weights of the positions.
 constexpr int kFinishWaves = 4, kFinishThreads = kWave * kFinishWaves;
 
-template <int kHs, int kPieces>
+template <int kHs, bool kByTiles>
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges, int mass_rounds) {
-    constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours;
+    constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours, kPieces = kByTiles ? 4 : 2, kOfWave = 16 * kPieces;
+    constexpr int kQueryBytes = Queries<kHs>::kLdsBytes > 0 ? Queries<kHs>::kLdsBytes : 16;
     __shared__ float weights[kMaxSplits];
     __shared__ __align__(16) float partial[kSlices][kHs];
-    __shared__ float tops[kRows], inverses[kRows];
     __shared__ __align__(16) char scale_lds[kFinishWaves][ScaleRows<kHs>::kLdsBytes];
-    __shared__ __align__(16) char q_lds[Queries<kHs>::kLdsBytes > 0 ? Queries<kHs>::kLdsBytes : 16];
+    __shared__ __align__(16) char q_lds[kByTiles ? kFinishWaves : 1][kQueryBytes];
+    __shared__ float of_waves[kFinishWaves][kOfWave];       // (by tiles)
+    __shared__ float tops[kRows], inverses[kRows];          // (one tile)
     const int lane = lane_id(), wave = wave_index(), column = lane & 15, part = lane >> 4;
     const int head = static_cast<int>(blockIdx.x % job.heads), block = static_cast<int>(blockIdx.x / job.heads);
     const int kvh = head % job.n_kv_heads, s = head / job.n_kv_heads, start = job.start_of(s), tokens = job.tokens();
@@ -472,10 +474,11 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         }
         return;
     }
-    // (rounds of kRound positions, one for each block of the sequence and head in turn)
-    constexpr int kOfWave = 16 * kPieces, kRound = kOfWave * kFinishWaves;
-    const int blocks = (all_end + kRound * mass_rounds - 1) / (kRound * mass_rounds);
-    const int p_first = (block - merges) * kRound;
+    // One tile: a round is kOfWave positions for each wavefront, and a block's rounds are taken in turn with the other blocks of the sequence and
+    // head.  Several tiles: kOfWave positions for all wavefronts, which take the tiles in turn (one after the other in every wavefront,
+    // what counts is the time of a tile's requests: 16 rows of 4 sequences of up to 3000 positions, heads of 64, 18 us and 14).
+    const int span = kByTiles ? kOfWave : kOfWave * kFinishWaves;
+    const int blocks = (all_end + span * mass_rounds - 1) / (span * mass_rounds);
     if (block - merges >= blocks) return;
     const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
     const uint32_t* codes = job.cache.codes[0] + head_rows * (kHs / 8);
@@ -484,27 +487,27 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
     const int columns = min(tokens, job.n_q) * job.shared;
     const Kv4Reader read;
-    const int last = all_end;
-    // (a wavefront has kOfWave neighbouring positions of a round)
     Piece<kHs> k[kPieces], next[kPieces];
     ScaleRows<kHs> pairs;
     char* pairs_lds = scale_lds[wave];
-    auto request = [&](int base) {
-        pairs.load(scales, min(base + kOfWave * wave + (lane & (kOfWave - 1)), last - 1));
+    const int offset = kByTiles ? 0 : kOfWave * wave, step = blocks * span;
+    auto request = [&](int p0) {
+        pairs.load(scales, min(p0 + (lane & (kOfWave - 1)), all_end - 1));
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) next[i].load(codes, min(base + kOfWave * wave + 16 * i + column, last - 1), part);
+        for (int i = 0; i < kPieces; ++i) next[i].load(codes, min(p0 + 16 * i + column, all_end - 1), part);
     };
-    request(p_first);
+    request((block - merges) * span + offset);
     Queries<kHs> q;
     float top = 0.0f, inverse = 0.0f;
     int loaded = -1;  // the tile that `q`, `top` and `inverse` are of
-    for (int base = p_first; base < last; base += blocks * kRound) {
+    for (int base = (block - merges) * span; base < all_end; base += step) {
+        const int p0 = base + offset;
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) k[i] = next[i];
         pairs.put(pairs_lds);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) k[i].pair = ScaleRows<kHs>::get(pairs_lds, 16 * i + column, part);
-        if (base + blocks * kRound < last) request(base + blocks * kRound);
+        if (base + step < all_end) request(p0 + step);
         floatx4 sum[kPieces];  // of this lane's column, over the tiles
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) sum[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -512,45 +515,71 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         float before[kPieces];
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
-            const int p = base + kOfWave * wave + 16 * i + 4 * part + column;
-            before[i] = column < 4 && p < last ? mass[p] : 0.0f;
+            const int p = p0 + 16 * i + 4 * part + column;
+            before[i] = !kByTiles && column < 4 && p < all_end ? mass[p] : 0.0f;
         }
-        for (int tile = 0; tile < job.tiles; ++tile) {
-            if (job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1) <= base) continue;  // (uniform)
+        for (int tile = kByTiles ? wave : 0; tile < job.tiles; tile += kFinishWaves) {
+            const int tile_end = job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1);
+            if (kByTiles && tile_end <= p0) continue;  // (uniform in the wavefront; one tile: the block's barrier is ahead)
             const Column mine(job, tile, column);
             const int my_end = mine.valid ? job.end_of(start, mine.token) : 0;
             if (loaded != tile) {
-                if (loaded >= 0) __syncthreads();  // (the tile before is done with what LDS holds)
                 loaded = tile;
-                q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds, wave, kFinishWaves);
-                // (maximum, 1 / sum) of the tile's rows: 16 threads to a row
                 const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
-                const int row = threadIdx.x / 16, at = threadIdx.x % 16;
-                const bool live = row < min(tokens, job.n_q - tile * tokens) * job.shared;
-                float2 st[kMaxSplits / 16];
-                float highest = -INFINITY, total = 0.0f;
+                if constexpr (kByTiles) {
+                    q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds[wave], 0, 1);
+                    // (maximum, 1 / sum) of this lane's column: the shares' in four parts, which meet across the lanes that have the column
+                    top = -INFINITY;
+                    float total = 0.0f;
+                    for (int i0 = 0; i0 < active; i0 += 16) {
+                        float2 st[4];
+                        float highest = top;
 #pragma unroll
-                for (int i = 0; i < kMaxSplits / 16; ++i) {
-                    st[i] = make_float2(-INFINITY, 0.0f);
-                    if (live && at + 16 * i < active) st[i] = job.stats[(slot + at + 16 * i) * kRows + row];
-                    highest = fmaxf(highest, st[i].x);
-                }
-                highest = fmaxf(highest, dpp_move<kDppXor1>(highest));
-                highest = fmaxf(highest, dpp_move<kDppXor2>(highest));
-                highest = fmaxf(highest, dpp_move<kDppHalfMirror>(highest));
-                highest = fmaxf(highest, dpp_move<kDppMirror>(highest));
-                if (highest == -INFINITY) highest = 0.0f;
+                        for (int j = 0; j < 4; ++j) {
+                            const int at = i0 + 4 * j + part;
+                            st[j] = mine.valid && at < active ? job.stats[(slot + at) * kRows + column] : make_float2(-INFINITY, 0.0f);
+                            highest = fmaxf(highest, st[j].x);
+                        }
+                        const float reference = highest == -INFINITY ? 0.0f : highest;
+                        total *= __builtin_amdgcn_exp2f(top - reference);
 #pragma unroll
-                for (int i = 0; i < kMaxSplits / 16; ++i) total = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - highest), total);
-                total = row16_sum(total);
-                if (at == 0) {
-                    tops[row] = highest;
-                    inverses[row] = 1.0f / total;
+                        for (int j = 0; j < 4; ++j) total = fmaf(st[j].y, __builtin_amdgcn_exp2f(st[j].x - reference), total);
+                        top = highest;
+                    }
+                    const float highest = rows_max(top), reference = highest == -INFINITY ? 0.0f : highest;
+                    total = rows_sum(total * __builtin_amdgcn_exp2f(top - reference));
+                    top = reference;
+                    inverse = 1.0f / total;
+                } else {
+                    q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds[0], wave, kFinishWaves);
+                    // (maximum, 1 / sum) of the tile's rows: 16 threads to a row
+                    const int row = threadIdx.x / 16, at = threadIdx.x % 16;
+                    float2 st[kMaxSplits / 16];
+                    float highest = -INFINITY, total = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kMaxSplits / 16; ++i) {
+                        st[i] = row < columns && at + 16 * i < active ? job.stats[(slot + at + 16 * i) * kRows + row] : make_float2(-INFINITY, 0.0f);
+                        highest = fmaxf(highest, st[i].x);
+                    }
+                    highest = fmaxf(highest, dpp_move<kDppXor1>(highest));
+                    highest = fmaxf(highest, dpp_move<kDppXor2>(highest));
+                    highest = fmaxf(highest, dpp_move<kDppHalfMirror>(highest));
+                    highest = fmaxf(highest, dpp_move<kDppMirror>(highest));
+                    if (highest == -INFINITY) highest = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kMaxSplits / 16; ++i) total = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - highest), total);
+                    total = row16_sum(total);
+                    if (at == 0) {
+                        tops[row] = highest;
+                        inverses[row] = 1.0f / total;
+                    }
+                    __syncthreads();
+                    top = tops[column];
+                    inverse = inverses[column];
                 }
-                __syncthreads();
-                top = tops[column];
-                inverse = inverses[column];
             }
+            // (uniform) a row does not attend to all of the positions, or there is no row
+            const bool partly = p0 + kOfWave > job.end_of(start, tile * tokens) || columns < kRows || (tile + 1) * tokens > job.n_q;
 #pragma unroll
             for (int i = 0; i < kPieces; i += 2) {
                 floatx4 st[2];
@@ -559,8 +588,9 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -top)) * inverse;
-                        sum[i + t][e] += base + kOfWave * wave + 16 * (i + t) + 4 * part + e < my_end ? w : 0.0f;
+                        float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -top)) * inverse;
+                        if (partly) w = p0 + 16 * (i + t) + 4 * part + e < my_end ? w : 0.0f;
+                        sum[i + t][e] += w;
                     }
             }
         }
@@ -578,8 +608,22 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
                     sum[i][e] += dpp_move<kDppMirror>(sum[i][e]);
                 }
             }
-            const int p = base + kOfWave * wave + 16 * i + 4 * part + column;
-            if (column < 4 && p < last) mass[p] = before[i] + (column == 0 ? sum[i][0] : column == 1 ? sum[i][1] : column == 2 ? sum[i][2] : sum[i][3]);
+            const float mine = column == 0 ? sum[i][0] : column == 1 ? sum[i][1] : column == 2 ? sum[i][2] : sum[i][3];
+            const int at = 16 * i + 4 * part + column;
+            if (column < 4) {
+                if (kByTiles) of_waves[wave][at] = mine;
+                else if (p0 + at < all_end) mass[p0 + at] = before[i] + mine;
+            }
+        }
+        if constexpr (kByTiles) {
+            __syncthreads();
+            if (threadIdx.x < kOfWave && base + static_cast<int>(threadIdx.x) < all_end) {
+                float total = mass[base + threadIdx.x];
+#pragma unroll
+                for (int w = 0; w < kFinishWaves; ++w) total += of_waves[w][threadIdx.x];
+                mass[base + threadIdx.x] = total;
+            }
+            __syncthreads();
         }
     }
 }
@@ -691,18 +735,17 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     else
         LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
     const int merges = job.splits > 1 ? job.tiles * kRows : 0;
-    // The account: several tiles (more than 16 rows) take 256 positions at a time, K once for all of them, and one such round to a block: what
-    // counts is how often a tile's queries are read.  One tile: 128 at a time, and as many rounds to a block, up to 8, as leave three blocks
-    // to a compute unit.
-    const int round = job.tiles > 1 ? 256 : 128;
+    // The account's blocks: one tile of rows: as many rounds of 128 positions to a block, up to 8, as leave three blocks to a compute unit; several:
+    // 64 positions to a block.
+    const int round = job.tiles > 1 ? 64 : 128;
     const long long rounds = (static_cast<long long>(shape->seq_len) + round - 1) / round * job.heads / (3 * compute_units());
     const int mass_rounds = job.tiles > 1 || rounds < 1 ? 1 : rounds < 8 ? static_cast<int>(rounds) : 8;
     const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + round * mass_rounds - 1) / (round * mass_rounds) : 0);
     if (blocks > 0) {
         LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch",
                     job.heads, shape->seq_len);
-        const auto kernel = shape->head_size == 64 ? (job.tiles > 1 ? &finish_kernel<64, 4> : &finish_kernel<64, 2>)
-                                                   : (job.tiles > 1 ? &finish_kernel<128, 4> : &finish_kernel<128, 2>);
+        const auto kernel = shape->head_size == 64 ? (job.tiles > 1 ? &finish_kernel<64, true> : &finish_kernel<64, false>)
+                                                   : (job.tiles > 1 ? &finish_kernel<128, true> : &finish_kernel<128, false>);
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, merges, mass_rounds);
         LPP_CHECK_LAUNCH("finish_kernel");
     }
