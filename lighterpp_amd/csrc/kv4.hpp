@@ -85,5 +85,22 @@ struct Kv4Reader {
     }
 };
 
+// How many of n values that do not decrease, value(0) .. value(n - 1), are at or below `limit`.  The whole wavefront looks at 64 of them at a time:
+// one round for up to 64, two for 4096.
+template <typename Value>
+__device__ __forceinline__ int count_up_to(int n, int limit, Value value) {
+    int from = 0, count = n;  // the first `from` are; none behind the first from + count is
+    while (count > 0) {
+        const int step = (count + kWave - 1) / kWave, at = from + step * lane_id() + step - 1;
+        const bool is = at < from + count && value(at) <= limit;
+        const int blocks = __popcll(__builtin_amdgcn_ballot_w64(is));
+        const int left = count - step * blocks;
+        from += step * blocks;
+        count = step == 1 ? 0 : min(left, step - 1);
+        if (blocks == kWave) break;
+    }
+    return from;
+}
+
 }  // namespace dev
 }  // namespace lpp

@@ -93,22 +93,20 @@ __global__ __launch_bounds__(kStoreThreads) void store_kernel(Kv4Layer to, const
     };
     request(0);
     int s = 0, first = 0, start = 0;
-    if (offsets != nullptr) {
-        int begin = offsets[0];
-        for (;; s += kWave) {
-            if (s >= n_seqs) return;
-            const int at = min(s + lane, n_seqs - 1);
-            const int end = offsets[at + 1], its_start = starts != nullptr ? starts[at] : 0;
-            const int ended = __popcll(__builtin_amdgcn_ballot_w64(end <= row && s + lane < n_seqs));
-            if (ended > 0) begin = __builtin_amdgcn_readlane(end, ended - 1);
-            if (ended == kWave) continue;
-            s += ended;
-            if (s >= n_seqs) return;
-            start = __builtin_amdgcn_readlane(its_start, ended);
-            break;
-        }
-        first = max(begin, 0);
+    if (offsets != nullptr && n_seqs > kWave) {
+        s = count_up_to(n_seqs, row, [&](int at) { return offsets[at + 1]; });
+        if (s >= n_seqs) return;
+        first = max(offsets[s], 0);
         if (row < first) return;
+        if (starts != nullptr) start = starts[s];
+    } else if (offsets != nullptr) {
+        const int at = min(lane, n_seqs - 1);
+        const int begin = offsets[0], end = offsets[at + 1], its_start = starts != nullptr ? starts[at] : 0;
+        s = __popcll(__builtin_amdgcn_ballot_w64(end <= row && lane < n_seqs));
+        if (s >= n_seqs) return;
+        first = max(s > 0 ? __builtin_amdgcn_readlane(end, s > 0 ? s - 1 : 0) : begin, 0);
+        if (row < first) return;
+        start = __builtin_amdgcn_readlane(its_start, s);
     } else {
         const int each = n_tokens / n_seqs;
         s = row / each;
@@ -417,6 +415,9 @@ lpp_status lpp_kv4_store(void* d_cache, const lpp_kv4_shape* shape, int layer, c
     const int per16 = type == LPP_F32 ? 4 : 8;
     LPP_REQUIRE(reinterpret_cast<uintptr_t>(d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(d_v) % 16 == 0 && kv_stride % per16 == 0,
                 "lpp_kv4_store: rows of K and V must start at multiples of 16 bytes");
+    const size_t in_bytes = (static_cast<size_t>(n_tokens - 1) * kv_stride + kv_dim) * (type == LPP_F32 ? 4 : 2);
+    LPP_REQUIRE(!ranges_overlap(d_k, in_bytes, d_cache, kv4_bytes(*shape)) && !ranges_overlap(d_v, in_bytes, d_cache, kv4_bytes(*shape)),
+                "lpp_kv4_store: the rows overlap the cache");
     const Kv4Layer to = kv4_layer(d_cache, *shape, layer);
     const dim3 grid((static_cast<unsigned>(n_tokens) + kStoreThreads / dev::kWave - 1) / (kStoreThreads / dev::kWave));
     if (type == LPP_F32)
@@ -465,7 +466,7 @@ lpp_status lpp_kv4_evict(void* d_dst, const lpp_kv4_shape* dst, int dst_layer, f
     LPP_REQUIRE(recent >= 0 && recent <= keep && keep > 0 && keep <= dst->seq_len, "lpp_kv4_evict: keep = %d, recent = %d, room for %d", keep, recent,
                 dst->seq_len);
     const long long planes = static_cast<long long>(dst->n_seqs) * dst->n_kv_heads;
-    LPP_REQUIRE(planes <= 0x7fffffffll, "lpp_kv4_evict: %lld sequences times KV heads", planes);
+    LPP_REQUIRE(planes * kSelectThreads < (1ll << 32), "lpp_kv4_evict: %lld sequences times KV heads", planes);
     LPP_REQUIRE(!ranges_overlap(d_dst, kv4_bytes(*dst), d_src, kv4_bytes(*src)), "lpp_kv4_evict: the caches overlap");
     const size_t dst_mass_bytes = kv4_layer_rows(*dst) * dst->n_layers * 4, src_mass_bytes = kv4_layer_rows(*src) * src->n_layers * 4;
     LPP_REQUIRE(!ranges_overlap(d_dst_mass, dst_mass_bytes, d_mass, src_mass_bytes), "lpp_kv4_evict: d_dst_mass overlaps d_mass");

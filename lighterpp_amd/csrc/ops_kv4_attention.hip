@@ -33,10 +33,12 @@ struct AttendJob {
     __device__ __forceinline__ int end_of(int start, int row) const { return min(max(start + row + 1, 0), seq_len); }
     __device__ __forceinline__ int tokens() const { return static_cast<int>(kRows * per_shared >> 16); }  // of a tile
     // How many shares a sequence's `positions` are cut into: of all sequences' positions, as many to each as gives `workgroups` of them in all,
-    // but no fewer than `least`.  (All lanes call it and read the sequences' starts, 64 at a time; the same sum in every workgroup.)
+    // but no fewer than `least`.  (All lanes call it and read the sequences' starts, 64 at a time; the same sum in every workgroup.  Of very many
+    // sequences all are taken to be as long as this one.)
     __device__ __forceinline__ int shares_of(int positions) const {
-        float all = 0.0f;
-        for (int s0 = 0; s0 < n_seqs; s0 += kWave) all += wave_sum(s0 + lane_id() < n_seqs ? static_cast<float>(end_of(start_of(s0 + lane_id()), n_q - 1)) : 0.0f);
+        float all = n_seqs > 4 * kWave ? static_cast<float>(positions) * n_seqs : 0.0f;
+        if (n_seqs <= 4 * kWave)
+            for (int s0 = 0; s0 < n_seqs; s0 += kWave) all += wave_sum(s0 + lane_id() < n_seqs ? static_cast<float>(end_of(start_of(s0 + lane_id()), n_q - 1)) : 0.0f);
         const int each = max(least, static_cast<int>(fminf(all * per_workgroup, 1e9f)));
         return max(min((positions + each - 1) / each, splits), 1);
     }
@@ -433,7 +435,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
     const int active = job.shares_of(all_end);
     if (block < merges) {
         if (active == 1) return;
-        const int tile = block / kRows, row = block % kRows;
+        const int rows = min(tokens, job.n_q) * job.shared, tile = block / rows, row = block % rows;
         const Column its(job, tile, row);
         if (!its.valid) return;
         const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
@@ -643,8 +645,10 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
     s.waves = heads * 4 > compute_units() ? 4 : 8;
     s.least = 512;
     s.workgroups = compute_units() * (shape.head_size == 64 ? 16 / s.waves : s.waves == 8 ? 1 : 3);  // (by registers, and LDS for the heads of 128)
-    const int most = (shape.seq_len + s.least - 1) / s.least;
-    s.splits = most < kMaxSplits ? most : kMaxSplits;
+    // (no more workgroups than 16 rounds of them, most of which would find no share)
+    const long long rounds = 16ll * s.workgroups / heads, most = (shape.seq_len + s.least - 1) / s.least;
+    s.splits = static_cast<int>(most < kMaxSplits ? most : kMaxSplits);
+    if (s.splits > rounds) s.splits = static_cast<int>(rounds > 1 ? rounds : 1);
     return s;
 }
 
@@ -706,6 +710,9 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     LPP_REQUIRE(workspace_bytes >= need, "lpp_kv4_attention: a workspace of %zu bytes, %zu are needed", workspace_bytes, need);
     const size_t rows_bytes = static_cast<size_t>(shape->n_seqs) * n_q * n_heads * shape->head_size * 4;
     LPP_REQUIRE(!ranges_overlap(d_out, rows_bytes, d_q, rows_bytes), "lpp_kv4_attention: d_out overlaps d_q");
+    LPP_REQUIRE(!ranges_overlap(d_workspace, need, d_q, rows_bytes) && !ranges_overlap(d_workspace, need, d_out, rows_bytes) &&
+                    !ranges_overlap(d_workspace, need, d_cache, kv4_bytes(*shape)),
+                "lpp_kv4_attention: the workspace overlaps q, out or the cache");
     AttendJob job;
     job.out = d_out;
     job.q = d_q;
@@ -734,7 +741,7 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
         LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
     else
         LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
-    const int merges = job.splits > 1 ? job.tiles * kRows : 0;
+    const int merges = job.splits > 1 ? job.tiles * (n_q < kRows / job.shared ? n_q : kRows / job.shared) * job.shared : 0;
     // The account's blocks: one tile of rows: as many rounds of 128 positions to a block, up to 8, as leave three blocks to a compute unit; several:
     // 64 positions to a block.
     const int round = job.tiles > 1 ? 64 : 128;

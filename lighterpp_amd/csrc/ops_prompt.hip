@@ -62,52 +62,45 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
 
 __device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_readlane(wave_inclusive_sum(v), kWave - 1); }
 
-// The `tile`-th of all sequences' tiles: which of its sequence's tiles it is, and the sequence's rows (returned; 0: there are not as many
-// tiles).  Up to 64 sequences: in the order of their walks' lengths, longest first, whatever the sequence; more: one sequence
-// after the other, each from its last tile.
+// The workgroup's tile: which of its sequence's tiles it is, and the sequence's rows (returned; 0: it has none).  Up to 64 sequences: in the order of
+// their walks' lengths, longest first, whatever the sequence.  More: sequence s's tiles, the last one first, from number
+// offsets[s] / tokens + s on, which leaves room for those of the sequences before.
 __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& tile, int& first_row) {
     if (job.offsets == nullptr) {
         first_row = 0;
         tile = (job.n_tokens + tokens - 1) / tokens - 1 - tile;
         return tile >= 0 ? job.n_tokens : 0;
     }
-    const int lane = lane_id();
-    for (int s0 = 0; s0 < job.n_seqs; s0 += kWave) {
-        const int s = s0 + lane;
-        const int begin = s < job.n_seqs ? min(max(job.offsets[s], 0), job.n_tokens) : 0;
-        const int end = s < job.n_seqs ? min(max(job.offsets[s + 1], 0), job.n_tokens) : 0;
-        const int rows = max(end - begin, 0), tiles = (rows + tokens - 1) / tokens;
-        if (job.n_seqs <= kWave) {
-            // tile number `level` of every sequence that has one, from the highest level down: the level with as many tiles above it as
-            // are before this one
-            if (wave_sum_int(tiles) <= tile) return 0;
-            int low = 0, high = static_cast<int>(wave_max(static_cast<float>(min(tiles, 1 << 24))));  // at and above `low` more tiles than `tile`, at `high` not
-            if (high == 1 << 24) high = (job.n_tokens + tokens - 1) / tokens;
-            while (high - low > 1) {
-                const int middle = (low + high) / 2;
-                if (wave_sum_int(max(tiles - middle, 0)) > tile) low = middle;
-                else high = middle;
-            }
-            const int rank = tile - wave_sum_int(max(tiles - low - 1, 0));
-            const unsigned long long there = __builtin_amdgcn_ballot_w64(tiles > low);
-            const int before = __popcll(there & ((1ull << lane) - 1ull));
-            const unsigned long long mine = __builtin_amdgcn_ballot_w64(tiles > low && before == rank);
-            const int at = __builtin_ctzll(mine);
-            first_row = __builtin_amdgcn_readlane(begin, at);
-            tile = low;
-            return __builtin_amdgcn_readlane(rows, at);
-        }
-        const int upto = wave_inclusive_sum(tiles);
-        const unsigned long long behind = __builtin_amdgcn_ballot_w64(upto > tile);
-        if (behind != 0ull) {
-            const int at = __builtin_ctzll(behind);
-            first_row = __builtin_amdgcn_readlane(begin, at);
-            tile = __builtin_amdgcn_readlane(upto, at) - 1 - tile;
-            return __builtin_amdgcn_readlane(rows, at);
-        }
-        tile -= __builtin_amdgcn_readlane(upto, kWave - 1);
+    const auto offset = [&](int s) { return min(max(job.offsets[s], 0), job.n_tokens); };
+    if (job.n_seqs > kWave) {
+        const int s = count_up_to(job.n_seqs, tile, [&](int at) { return offset(at) / tokens + at; }) - 1;
+        if (s < 0) return 0;
+        const int begin = __builtin_amdgcn_readfirstlane(offset(s)), end = __builtin_amdgcn_readfirstlane(offset(s + 1));
+        first_row = begin;
+        tile = (end - begin + tokens - 1) / tokens - 1 - (tile - begin / tokens - s);
+        return end - begin;
     }
-    return 0;
+    const int s = lane_id();
+    const int begin = s < job.n_seqs ? offset(s) : 0, end = s < job.n_seqs ? offset(s + 1) : 0;
+    const int rows = max(end - begin, 0), tiles = (rows + tokens - 1) / tokens;
+    // Tile number `level` of every sequence that has one, from the highest level down: the lowest level with more than `tile` tiles at and above it.
+    if (wave_sum_int(tiles) <= tile) return 0;
+    int low = 0, high = (job.n_tokens + tokens - 1) / tokens;  // at and above `low` there are more than `tile`, at and above `high` there are not
+    if (high > 64) high = static_cast<int>(wave_max(static_cast<float>(tiles))) + (high > 1 << 24 ? 128 : 0);
+    while (high - low > 1) {
+        const int middle = (low + high) / 2;
+        if (wave_sum_int(max(tiles - middle, 0)) > tile) low = middle;
+        else high = middle;
+    }
+    const int rank = tile - wave_sum_int(max(tiles - low - 1, 0));
+    const unsigned long long there = __builtin_amdgcn_ballot_w64(tiles > low);
+    const int before = __popcll(there & ((1ull << s) - 1ull));
+    const unsigned long long mine = __builtin_amdgcn_ballot_w64(tiles > low && before == rank);
+    if (mine == 0ull) return 0;  // (offsets that decrease)
+    const int at = __builtin_ctzll(mine);
+    first_row = __builtin_amdgcn_readlane(begin, at);
+    tile = low;
+    return __builtin_amdgcn_readlane(rows, at);
 }
 
 template <typename T, int kHs, int kR, int kP, int kStepRows>

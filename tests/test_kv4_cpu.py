@@ -44,7 +44,7 @@ def test_shapes_refused(lib, dims):
 
 def test_store_refused(lib):
     s = Shape(2, 3, 2, 10, 64)
-    call = lambda cache=P, layer=0, k=P, v=P, type=0, stride=128, offsets=None, n=6, starts=None: \
+    call = lambda cache=P, layer=0, k=2 * P, v=3 * P, type=0, stride=128, offsets=None, n=6, starts=None: \
         lib.lpp_kv4_store(cache, s, layer, k, v, type, stride, offsets, n, starts)  # noqa: E731
     assert call(n=0) == capi.LPP_OK and call(n=0, k=None, v=None) == capi.LPP_OK
     refused(lib, call(cache=None), b"null cache")
@@ -59,7 +59,8 @@ def test_store_refused(lib):
     refused(lib, call(stride=127), b"kv_stride")
     refused(lib, call(stride=130), b"16 bytes")
     refused(lib, call(type=1, stride=132), b"16 bytes")
-    refused(lib, call(k=P + 8), b"16 bytes")
+    refused(lib, call(k=4 * P + 8), b"16 bytes")
+    refused(lib, call(v=P + 1024), b"overlap")
 
 
 def test_load_refused(lib):
@@ -96,6 +97,9 @@ def test_attention_refused(lib):
     refused(lib, call(n_q=11), b"n_q")
     refused(lib, call(size=need.value - 1), b"workspace")
     refused(lib, call(out=2 * P + 16), b"overlap")
+    refused(lib, call(work=2 * P + 64), b"workspace")
+    refused(lib, call(work=P - 64), b"workspace")
+    refused(lib, call(work=3 * P + 64), b"workspace")
     for name in ("out", "q", "work"):
         refused(lib, call(**{name: 5 * P + 4}), b"16 bytes")
     refused(lib, lib.lpp_kv4_attention_workspace(s, 8, 2, None), b"null output")

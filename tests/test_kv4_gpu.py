@@ -83,6 +83,22 @@ def test_store_byte_for_byte(lib, rows, offsets, starts, hs, kv, typ):
     same_bytes(dcache, cache)
 
 
+@pytest.mark.parametrize("n_seqs", [64, 65, 300, 5000])
+def test_store_many_sequences(lib, n_seqs):
+    rng = np.random.default_rng(n_seqs)
+    lengths = rng.integers(0, 4, n_seqs)
+    lengths[:3] = lengths[n_seqs // 2:n_seqs // 2 + 20] = 0
+    offsets = 2 + np.concatenate([[0], np.cumsum(lengths)])
+    rows = int(offsets[-1]) + 3
+    starts = rng.integers(-1, 4, n_seqs)
+    shape, cache = Shape(1, n_seqs, 1, 5, 64), ko.Cache(1, n_seqs, 1, 5, 64, fill=0x3C)
+    dcache = DB.from_numpy(cache.buffer)
+    k, v = rng.standard_normal((rows, 1, 64)).astype(F), rng.standard_normal((rows, 1, 64)).astype(F)
+    store(lib, dcache, shape, 0, k, v, offsets, starts)
+    host_store(cache, 0, k, v, offsets, starts)
+    same_bytes(dcache, cache)
+
+
 def test_store_values_on_borders_and_extreme_groups(lib):
     """Values exactly between two codes (ties go to the even one), one step either side of them, constant groups, subnormal scales, the
     ends of the range, and everything beyond."""
@@ -261,6 +277,19 @@ def test_more_sequences_than_compute_units(lib):
     mass = np.zeros((1, seqs, kv, 150), F)
     got, got_mass = attend(lib, dcache, cache, 0, q, lengths - 1, mass)
     check_attention(got, got_mass, cache, 0, q, lengths - 1, mass)
+
+
+@pytest.mark.parametrize("n_seqs,n_q", [(300, 1), (300, 5), (2000, 1)])
+def test_very_many_sequences(lib, n_seqs, n_q):
+    rng = np.random.default_rng(n_seqs + n_q)
+    room = 40 if n_seqs > 1000 else 700
+    lengths = rng.integers(0, 30, n_seqs)
+    lengths[7], lengths[n_seqs - 1] = room, room - 1
+    cache = random_cache(rng, 1, n_seqs, 1, room, 64)
+    q = rng.standard_normal((n_seqs, n_q, 2, 64)).astype(F)
+    mass = np.zeros((1, n_seqs, 1, room), F)
+    got, got_mass = attend(lib, DB.from_numpy(cache.buffer), cache, 0, q, lengths - n_q, mass)
+    check_attention(got, got_mass, cache, 0, q, lengths - n_q, mass)
 
 
 @pytest.mark.parametrize("hs", [64, 128])

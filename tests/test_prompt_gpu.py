@@ -96,6 +96,26 @@ def test_many_short_sequences(lib, typ):
     against(run(lib, q, k, v, offsets), q, k, v, list(zip(offsets[:-1], offsets[1:])))
 
 
+def test_thousands_of_sequences(lib):
+    """More than a wavefront finds in two looks; a long one among them, empty stretches, rows of no sequence before, between none and behind."""
+    rng = np.random.default_rng(15)
+    lengths = rng.integers(0, 3, 5000)
+    lengths[1000:1100] = 0
+    lengths[2500], lengths[4999] = 300, 40
+    offsets = 7 + np.concatenate([[0], np.cumsum(lengths)])
+    rows = int(offsets[-1]) + 9
+    q, k, v = inputs(16, rows, 2, 1, 64, F)
+    got = run(lib, q, k, v, offsets)
+    assert np.all(got[:7] == F(7.25)) and np.all(got[-9:] == F(7.25))
+    check = [(a, b) for i, (a, b) in enumerate(zip(offsets[:-1], offsets[1:])) if b - a > 2 or i % 50 == 0]
+    for a, b in check:
+        if a < b:
+            want, _, tol = ko.attend_tolerance(q[a:b], k[a:b].transpose(1, 0, 2), v[a:b].transpose(1, 0, 2), [j + 1 for j in range(b - a)])
+            assert np.all(np.abs(got[a:b] - want) <= tol), (a, b)
+    single = offsets[:-1][lengths >= 1]  # a sequence's first row is its V row
+    assert np.all(np.abs(got[single] - v[single].astype(np.float64)) <= np.abs(v[single].astype(np.float64)) * 2.0 ** -20 + 1e-12)
+
+
 @pytest.mark.parametrize("typ", [F, H])
 def test_rows_outside_every_sequence_and_strides(lib, typ):
     """The first offset is not 0, the last is not the end; rows have space behind them."""
