@@ -13,7 +13,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 16;       // of a tile: (16 / shared) new rows x the query heads of a KV head
 constexpr int kStep = 32;       // positions a wavefront takes at a time
-constexpr int kMaxSplits = 64;  // ranges that a sequence's positions are cut into
+constexpr int kMaxSplits = 64;  // shares that a sequence's positions are cut into
 constexpr float kSlack = 6.0f;
 
 struct AttendJob {
@@ -22,8 +22,10 @@ struct AttendJob {
     Kv4Layer cache;
     const int* starts;
     float* mass;
-    float2* stats;     // [sequence][KV head][tile][range][16]: maximum (in powers of two) and sum of a range
-    float* partials;   // [sequence][KV head][tile][range][16][head_size]
+    float2* stats;     // [sequence][KV head][tile][share][rows]: maximum (in powers of two) and sum of a share
+    float* partials;   // [sequence][KV head][tile][share][rows][head_size]
+    float* scores;     // for the account: [sequence][KV head][step][rows][kStep]; null if there is none, or it is made from K again
+    int rows, steps;  // of a tile; that seq_len has
     unsigned heads;  // n_seqs times n_kv_heads
     int n_seqs, n_q, n_kv_heads, shared, seq_len, splits, least, tiles;
     float per_workgroup;  // KV heads times tiles over the workgroups there should be
@@ -242,6 +244,9 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         for (int i = 0; i < kWords; ++i) v_to[i] = column * kRowBytes + 16 * ((kWords * part + i) ^ swizzle(column));
     }
 
+    // (after the step's requests, so that none of those waits for these stores)
+    const bool keeps = job.scores != nullptr && mine.valid;
+    float* my_scores = job.scores + (static_cast<size_t>(head) * job.steps * job.rows + min(column, job.rows - 1)) * kStep + 4 * part;
     for (int p0 = first; p0 < end; p0 += stride) {
         const bool more = p0 + stride < end;         // (uniform)
         const bool partly = p0 + kStep > first_end;   // (uniform) some row does not attend to the whole step
@@ -272,6 +277,10 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st[t][e] = p0 + 16 * t + 4 * part + e < my_end ? st[t][e] : -INFINITY;
+        }
+        if (keeps) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) *reinterpret_cast<floatx4*>(my_scores + p0 * job.rows + 16 * t) = st[t];
         }
         float step_top = -INFINITY;
 #pragma unroll
@@ -408,9 +417,9 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
             for (int u = 0; u < 4; ++u) sum[u] = any ? sum[u] * inverse : 0.0f;
             *reinterpret_cast<floatx4*>(job.out + its.at(job, s, kvh) * kHs + 4 * four) = sum;
         } else {
-            *reinterpret_cast<floatx4*>(job.partials + (slot * kRows + row) * kHs + 4 * four) = sum;
+            *reinterpret_cast<floatx4*>(job.partials + (slot * job.rows + row) * kHs + 4 * four) = sum;
         }
-        if (four == 0) job.stats[slot * kRows + row] = make_float2(all_top, total);
+        if (four == 0) job.stats[slot * job.rows + row] = make_float2(all_top, total);
     }
 }
 
@@ -418,16 +427,44 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
 // the weights of the positions.
 constexpr int kFinishWaves = 4, kFinishThreads = kWave * kFinishWaves;
 
-template <int kHs, bool kByTiles>
-__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges, int mass_rounds) {
-    constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours, kPieces = kByTiles ? 4 : 2, kOfWave = 16 * kPieces;
+// Maximum and 1 / sum of a tile's rows, each in the lanes that have its column: the shares' in four parts, which meet across those lanes.
+struct Sums {
+    float top, inverse;
+    __device__ __forceinline__ void load(const AttendJob& job, int head, int tile, bool valid, int active) {
+        const int column = lane_id() & 15, part = lane_id() >> 4;
+        const float2* stats = job.stats + (static_cast<size_t>(head) * job.tiles + tile) * job.splits * job.rows + column;
+        float all = -INFINITY, total = 0.0f;
+        for (int i0 = 0; i0 < active; i0 += 16) {
+            float2 st[4];
+            float highest = all;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = i0 + 4 * j + part;
+                st[j] = valid && at < active ? stats[at * job.rows] : make_float2(-INFINITY, 0.0f);
+                highest = fmaxf(highest, st[j].x);
+            }
+            const float reference = highest == -INFINITY ? 0.0f : highest;
+            total *= __builtin_amdgcn_exp2f(all - reference);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) total = fmaf(st[j].y, __builtin_amdgcn_exp2f(st[j].x - reference), total);
+            all = highest;
+        }
+        const float highest = rows_max(all);
+        top = highest == -INFINITY ? 0.0f : highest;
+        inverse = 1.0f / rows_sum(total * __builtin_amdgcn_exp2f(all - top));
+    }
+};
+
+// kKept: the account is made from the scores that the shares have kept; else from K again.
+template <int kHs, bool kKept>
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges, int span) {
+    constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours, kPieces = 4, kOfWave = 16 * kPieces;
     constexpr int kQueryBytes = Queries<kHs>::kLdsBytes > 0 ? Queries<kHs>::kLdsBytes : 16;
     __shared__ float weights[kMaxSplits];
     __shared__ __align__(16) float partial[kSlices][kHs];
     __shared__ __align__(16) char scale_lds[kFinishWaves][ScaleRows<kHs>::kLdsBytes];
-    __shared__ __align__(16) char q_lds[kByTiles ? kFinishWaves : 1][kQueryBytes];
-    __shared__ float of_waves[kFinishWaves][kOfWave];       // (by tiles)
-    __shared__ float tops[kRows], inverses[kRows];          // (one tile)
+    __shared__ __align__(16) char q_lds[kFinishWaves][kQueryBytes];
+    __shared__ float of_waves[kFinishWaves][kOfWave];
     const int lane = lane_id(), wave = wave_index(), column = lane & 15, part = lane >> 4;
     const int head = static_cast<int>(blockIdx.x % job.heads), block = static_cast<int>(blockIdx.x / job.heads);
     const int kvh = head % job.n_kv_heads, s = head / job.n_kv_heads, start = job.start_of(s), tokens = job.tokens();
@@ -435,11 +472,11 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
     const int active = job.shares_of(all_end);
     if (block < merges) {
         if (active == 1) return;
-        const int rows = min(tokens, job.n_q) * job.shared, tile = block / rows, row = block % rows;
+        const int tile = block / job.rows, row = block % job.rows;
         const Column its(job, tile, row);
         if (!its.valid) return;
-        const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
-        // (the ranges' outputs are requested along with their weights; a range that the row does not attend to has left none)
+        const size_t slot = (static_cast<size_t>(head) * job.tiles + tile) * job.splits;
+        // (the shares' outputs are requested along with their weights; a share that the row does not attend to has left none)
         const int slice = static_cast<int>(threadIdx.x) / kFours, four = static_cast<int>(threadIdx.x) % kFours;
         constexpr int kEach = kMaxSplits / kSlices;
         floatx4 a[kEach];
@@ -447,9 +484,9 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         for (int i = 0; i < kEach; ++i) {
             if (kSlices * i >= active) break;  // (uniform)
             const int at = min(slice + kSlices * i, active - 1);
-            a[i] = *reinterpret_cast<const floatx4*>(job.partials + ((slot + at) * kRows + row) * kHs + 4 * four);
+            a[i] = *reinterpret_cast<const floatx4*>(job.partials + ((slot + at) * job.rows + row) * kHs + 4 * four);
         }
-        const float2 st = lane < active ? job.stats[(slot + lane) * kRows + row] : make_float2(-INFINITY, 0.0f);
+        const float2 st = lane < active ? job.stats[(slot + lane) * job.rows + row] : make_float2(-INFINITY, 0.0f);
         float top = wave_max(st.x);
         if (top == -INFINITY) top = 0.0f;
         const float weight = __builtin_amdgcn_exp2f(st.x - top);
@@ -476,112 +513,86 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
         }
         return;
     }
-    // One tile: a round is kOfWave positions for each wavefront, and a block's rounds are taken in turn with the other blocks of the sequence and
-    // head.  Several tiles: kOfWave positions for all wavefronts, which take the tiles in turn (one after the other in every wavefront,
-    // what counts is the time of a tile's requests: 16 rows of 4 sequences of up to 3000 positions, heads of 64, 18 us and 14).
-    const int span = kByTiles ? kOfWave : kOfWave * kFinishWaves;
-    const int blocks = (all_end + span * mass_rounds - 1) / (span * mass_rounds);
-    if (block - merges >= blocks) return;
-    const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
-    const uint32_t* codes = job.cache.codes[0] + head_rows * (kHs / 8);
-    const uint32_t* scales = job.cache.scales[0] + head_rows * (kHs / kKv4Group);
-    float* mass = job.mass + head_rows;
+    const int p_first = (block - merges) * span;
+    if (p_first >= all_end) return;
+    float* mass = job.mass + (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
-    const int columns = min(tokens, job.n_q) * job.shared;
-    const Kv4Reader read;
-    Piece<kHs> k[kPieces], next[kPieces];
-    ScaleRows<kHs> pairs;
-    char* pairs_lds = scale_lds[wave];
-    const int offset = kByTiles ? 0 : kOfWave * wave, step = blocks * span;
-    auto request = [&](int p0) {
-        pairs.load(scales, min(p0 + (lane & (kOfWave - 1)), all_end - 1));
+    Sums sums;
+    if constexpr (kKept) {
+        const float* scores = job.scores + static_cast<size_t>(head) * job.steps * job.rows * kStep;
+        // of a row whose lane has its sums: what a score adds to position p
+        auto weight = [&](float score, int row, int p, int row_end) {
+            const float top = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sums.top), row));
+            const float inverse = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sums.inverse), row));
+            return p < row_end ? __builtin_amdgcn_exp2f(fmaf(score, scale, -top)) * inverse : 0.0f;
+        };
+        // Four positions to a lane, four rows at a time, the next of them on their way.
+        typedef float Unaligned4 __attribute__((ext_vector_type(4), aligned(4)));
+        constexpr int kAt = 4, kOnce = 4 * kWave;
+        const int p_end = min(p_first + span, all_end);
+        floatx4 sc[kAt], now[kAt];
+        auto request = [&](int p0, int c0) {
+            const int at = min(p0 + 4 * lane, job.steps * kStep - 4);
+            const float* from = scores + static_cast<size_t>(at / kStep) * job.rows * kStep + at % kStep;
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) next[i].load(codes, min(p0 + 16 * i + column, all_end - 1), part);
-    };
-    request((block - merges) * span + offset);
-    Queries<kHs> q;
-    float top = 0.0f, inverse = 0.0f;
-    int loaded = -1;  // the tile that `q`, `top` and `inverse` are of
-    for (int base = (block - merges) * span; base < all_end; base += step) {
-        const int p0 = base + offset;
+            for (int c = 0; c < kAt; ++c) sc[c] = *reinterpret_cast<const floatx4*>(from + min(c0 + c, job.rows - 1) * kStep);
+        };
+        int p0 = p_first + kOnce * wave;
+        if (p0 >= p_end) return;  // (no barrier ahead)
+        request(p0, 0);
+        sums.load(job, head, 0, Column(job, 0, column).valid, active);
+        while (p0 < p_end) {  // (uniform in the wavefront)
+            const int p = p0 + 4 * lane;
+            const bool whole = p + 4 <= all_end;
+            floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f}, before = sum;
+            if (whole) before = *reinterpret_cast<const Unaligned4*>(mass + p);
+            p0 += kOnce * kFinishWaves;
+            for (int c0 = 0; c0 < job.rows; c0 += kAt) {
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) k[i] = next[i];
+                for (int c = 0; c < kAt; ++c) now[c] = sc[c];
+                if (c0 + kAt < job.rows) request(p - 4 * lane, c0 + kAt);
+                else if (p0 < p_end) request(p0, 0);
+#pragma unroll
+                for (int c = 0; c < kAt; ++c) {
+                    if (c0 + c >= job.rows) break;
+                    const int row_end = job.end_of(start, static_cast<int>((c0 + c) * job.per_shared >> 16));
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) sum[u] += weight(now[c][u], c0 + c, p + u, row_end);
+                }
+            }
+            if (whole) *reinterpret_cast<Unaligned4*>(mass + p) = before + sum;
+            else
+                for (int u = 0; u < 4; ++u)
+                    if (p + u < all_end) mass[p + u] += sum[u];
+        }
+    } else {
+        const size_t head_rows = (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
+        // One tile: the wavefronts take the positions in turn.  Several: each position's tiles (one after the other in every wavefront, what counts
+        // is the time of a tile's requests: 16 rows of 4 sequences of up to 3000 positions, heads of 64, 18 us and 14).
+        const bool by_tiles = job.tiles > 1;
+        const int p0 = p_first + (by_tiles ? 0 : kOfWave * wave);
+        const Kv4Reader read;
+        Piece<kHs> k[kPieces];
+        ScaleRows<kHs> pairs;
+        char* pairs_lds = scale_lds[wave];
+        pairs.load(job.cache.scales[0] + head_rows * (kHs / kKv4Group), min(p0 + lane, all_end - 1));
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) k[i].load(job.cache.codes[0] + head_rows * (kHs / 8), min(p0 + 16 * i + column, all_end - 1), part);
         pairs.put(pairs_lds);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) k[i].pair = ScaleRows<kHs>::get(pairs_lds, 16 * i + column, part);
-        if (base + step < all_end) request(p0 + step);
         floatx4 sum[kPieces];  // of this lane's column, over the tiles
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) sum[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        // (a lane adds the weights of one position a piece: position 4 part + column, for columns below four)
-        float before[kPieces];
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int p = p0 + 16 * i + 4 * part + column;
-            before[i] = !kByTiles && column < 4 && p < all_end ? mass[p] : 0.0f;
-        }
-        for (int tile = kByTiles ? wave : 0; tile < job.tiles; tile += kFinishWaves) {
-            const int tile_end = job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1);
-            if (kByTiles && tile_end <= p0) continue;  // (uniform in the wavefront; one tile: the block's barrier is ahead)
+        for (int tile = by_tiles ? wave : 0; tile < job.tiles; tile += by_tiles ? kFinishWaves : 1) {
+            if (job.end_of(start, min(tile * tokens + tokens, job.n_q) - 1) <= p0) continue;  // (uniform in the wavefront)
             const Column mine(job, tile, column);
             const int my_end = mine.valid ? job.end_of(start, mine.token) : 0;
-            if (loaded != tile) {
-                loaded = tile;
-                const size_t slot = ((static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.tiles + tile) * job.splits;
-                if constexpr (kByTiles) {
-                    q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds[wave], 0, 1);
-                    // (maximum, 1 / sum) of this lane's column: the shares' in four parts, which meet across the lanes that have the column
-                    top = -INFINITY;
-                    float total = 0.0f;
-                    for (int i0 = 0; i0 < active; i0 += 16) {
-                        float2 st[4];
-                        float highest = top;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int at = i0 + 4 * j + part;
-                            st[j] = mine.valid && at < active ? job.stats[(slot + at) * kRows + column] : make_float2(-INFINITY, 0.0f);
-                            highest = fmaxf(highest, st[j].x);
-                        }
-                        const float reference = highest == -INFINITY ? 0.0f : highest;
-                        total *= __builtin_amdgcn_exp2f(top - reference);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) total = fmaf(st[j].y, __builtin_amdgcn_exp2f(st[j].x - reference), total);
-                        top = highest;
-                    }
-                    const float highest = rows_max(top), reference = highest == -INFINITY ? 0.0f : highest;
-                    total = rows_sum(total * __builtin_amdgcn_exp2f(top - reference));
-                    top = reference;
-                    inverse = 1.0f / total;
-                } else {
-                    q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds[0], wave, kFinishWaves);
-                    // (maximum, 1 / sum) of the tile's rows: 16 threads to a row
-                    const int row = threadIdx.x / 16, at = threadIdx.x % 16;
-                    float2 st[kMaxSplits / 16];
-                    float highest = -INFINITY, total = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kMaxSplits / 16; ++i) {
-                        st[i] = row < columns && at + 16 * i < active ? job.stats[(slot + at + 16 * i) * kRows + row] : make_float2(-INFINITY, 0.0f);
-                        highest = fmaxf(highest, st[i].x);
-                    }
-                    highest = fmaxf(highest, dpp_move<kDppXor1>(highest));
-                    highest = fmaxf(highest, dpp_move<kDppXor2>(highest));
-                    highest = fmaxf(highest, dpp_move<kDppHalfMirror>(highest));
-                    highest = fmaxf(highest, dpp_move<kDppMirror>(highest));
-                    if (highest == -INFINITY) highest = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kMaxSplits / 16; ++i) total = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - highest), total);
-                    total = row16_sum(total);
-                    if (at == 0) {
-                        tops[row] = highest;
-                        inverses[row] = 1.0f / total;
-                    }
-                    __syncthreads();
-                    top = tops[column];
-                    inverse = inverses[column];
-                }
-            }
+            Queries<kHs> q;
+            q.load(job.q + mine.at(job, s, kvh) * kHs, part, q_lds[wave], 0, 1);
+            sums.load(job, head, tile, mine.valid, active);
             // (uniform) a row does not attend to all of the positions, or there is no row
-            const bool partly = p0 + kOfWave > job.end_of(start, tile * tokens) || columns < kRows || (tile + 1) * tokens > job.n_q;
+            const bool partly = p0 + kOfWave > job.end_of(start, tile * tokens) || job.rows < kRows || (tile + 1) * tokens > job.n_q;
 #pragma unroll
             for (int i = 0; i < kPieces; i += 2) {
                 floatx4 st[2];
@@ -590,7 +601,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -top)) * inverse;
+                        float w = __builtin_amdgcn_exp2f(fmaf(st[t][e], scale, -sums.top)) * sums.inverse;
                         if (partly) w = p0 + 16 * (i + t) + 4 * part + e < my_end ? w : 0.0f;
                         sum[i + t][e] += w;
                     }
@@ -599,34 +610,21 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sum[i][e] += dpp_move<kDppXor1>(sum[i][e]);
-                sum[i][e] += dpp_move<kDppXor2>(sum[i][e]);
-            }
-            if (columns > 4) {  // (uniform; columns that no row has have added nothing)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sum[i][e] += dpp_move<kDppHalfMirror>(sum[i][e]);
-                    sum[i][e] += dpp_move<kDppMirror>(sum[i][e]);
-                }
-            }
+            for (int e = 0; e < 4; ++e) sum[i][e] = row16_sum(sum[i][e]);
             const float mine = column == 0 ? sum[i][0] : column == 1 ? sum[i][1] : column == 2 ? sum[i][2] : sum[i][3];
-            const int at = 16 * i + 4 * part + column;
-            if (column < 4) {
-                if (kByTiles) of_waves[wave][at] = mine;
-                else if (p0 + at < all_end) mass[p0 + at] = before[i] + mine;
-            }
+            if (column < 4) of_waves[wave][16 * i + 4 * part + column] = mine;
         }
-        if constexpr (kByTiles) {
-            __syncthreads();
-            if (threadIdx.x < kOfWave && base + static_cast<int>(threadIdx.x) < all_end) {
-                float total = mass[base + threadIdx.x];
+        __syncthreads();
+        const int p = p_first + static_cast<int>(threadIdx.x);
+        if (static_cast<int>(threadIdx.x) >= span || p >= all_end) return;
+        float total = 0.0f;
+        if (by_tiles) {
 #pragma unroll
-                for (int w = 0; w < kFinishWaves; ++w) total += of_waves[w][threadIdx.x];
-                mass[base + threadIdx.x] = total;
-            }
-            __syncthreads();
+            for (int w = 0; w < kFinishWaves; ++w) total += of_waves[w][threadIdx.x];
+        } else {
+            total = of_waves[wave][lane];
         }
+        mass[p] += total;
     }
 }
 
@@ -651,6 +649,27 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
     if (s.splits > rounds) s.splits = static_cast<int>(rounds > 1 ? rounds : 1);
     return s;
 }
+
+// What the workspace holds.  Scores kept for the account are 4 bytes for every position and row; made from K again they cost its bytes and the
+// products (32 sequences of up to 8000 positions, 4 rows to a KV head of 128: 49 us more than without an account, and 14 so).  Not of several tiles, whose
+// scores are many times a layer (16 rows of 32 heads, 4 sequences of up to 3000 positions, heads of 64: 27.5 us for 25.5), and only where
+// the workspace gets no larger than partial results of kMaxSplits shares would make it: up to 14000 positions with four rows to a KV head of 64,
+// 2000 with sixteen.
+struct Workspace {
+    size_t stats, partials, scores;  // floats
+    int rows, steps;
+    size_t bytes() const { return (stats + partials + scores) * sizeof(float); }
+    Workspace(const lpp_kv4_shape& shape, int n_q, int shared, int tiles, int splits) {
+        const size_t all_tiles = static_cast<size_t>(shape.n_seqs) * shape.n_kv_heads * tiles;
+        rows = (n_q < kRows / shared ? n_q : kRows / shared) * shared;
+        steps = (shape.seq_len + kStep - 1) / kStep;
+        const size_t slots = static_cast<size_t>(splits) * rows, kept = static_cast<size_t>(rows) * steps * kStep;
+        const size_t sums = (slots * 2 + 3) / 4 * 4, outputs = slots * shape.head_size;
+        stats = all_tiles * sums;
+        partials = all_tiles * outputs;
+        scores = tiles == 1 && kept + sums + outputs <= static_cast<size_t>(kMaxSplits) * kRows * (shape.head_size + 2) ? all_tiles * kept : 0;
+    }
+};
 
 template <int kHs, int kWaves>
 lpp_status launch_attend(const AttendJob& job, dim3 grid) {
@@ -692,8 +711,7 @@ lpp_status lpp_kv4_attention_workspace(const lpp_kv4_shape* shape, int n_heads, 
     LPP_TRY(check("lpp_kv4_attention_workspace", shape, n_heads, n_q));
     LPP_REQUIRE(bytes != nullptr, "lpp_kv4_attention_workspace: null output");
     const int tiles = tiles_of(n_q, n_heads / shape->n_kv_heads);
-    const size_t slots = static_cast<size_t>(shape->n_seqs) * shape->n_kv_heads * tiles * split_of(*shape, tiles).splits;
-    *bytes = slots * kRows * (sizeof(float2) + shape->head_size * sizeof(float));
+    *bytes = Workspace(*shape, n_q, n_heads / shape->n_kv_heads, tiles, split_of(*shape, tiles).splits).bytes();
     return LPP_OK;
 }
 
@@ -731,9 +749,12 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     job.least = split.least;
     job.per_workgroup = static_cast<float>(shape->n_kv_heads) * job.tiles / split.workgroups;
     job.per_shared = (65536u + job.shared - 1) / job.shared;
-    const size_t slots = static_cast<size_t>(shape->n_seqs) * shape->n_kv_heads * job.tiles * job.splits;
+    const Workspace parts(*shape, n_q, job.shared, job.tiles, job.splits);
+    job.rows = parts.rows;
+    job.steps = parts.steps;
     job.stats = static_cast<float2*>(d_workspace);
-    job.partials = reinterpret_cast<float*>(job.stats + slots * kRows);
+    job.partials = static_cast<float*>(d_workspace) + parts.stats;
+    job.scores = d_mass != nullptr && parts.scores > 0 ? job.partials + parts.partials : nullptr;
     const long long groups = static_cast<long long>(job.heads) * job.tiles * job.splits;
     LPP_REQUIRE(groups * dev::kWave * split.waves < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads and %d rows are too many for a launch", job.heads, n_q);
     const dim3 grid(static_cast<unsigned>(groups));
@@ -741,19 +762,22 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
         LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
     else
         LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
-    const int merges = job.splits > 1 ? job.tiles * (n_q < kRows / job.shared ? n_q : kRows / job.shared) * job.shared : 0;
-    // The account's blocks: one tile of rows: as many rounds of 128 positions to a block, up to 8, as leave three blocks to a compute unit; several:
-    // 64 positions to a block.
-    const int round = job.tiles > 1 ? 64 : 128;
-    const long long rounds = (static_cast<long long>(shape->seq_len) + round - 1) / round * job.heads / (3 * compute_units());
-    const int mass_rounds = job.tiles > 1 || rounds < 1 ? 1 : rounds < 8 ? static_cast<int>(rounds) : 8;
-    const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + round * mass_rounds - 1) / (round * mass_rounds) : 0);
+    const int merges = job.splits > 1 ? job.tiles * job.rows : 0;
+    // The positions of one of the account's blocks.  From kept scores of one tile: as many rounds of 1024, up to 8, as leave four blocks to a compute
+    // unit.
+    const bool kept = job.scores != nullptr;
+    int span = job.tiles > 1 ? kWave : (kept ? 4 : 1) * kFinishThreads;
+    if (kept) {
+        const long long each = (static_cast<long long>(shape->seq_len) + span - 1) / span * job.heads / (4 * compute_units());
+        span *= each < 1 ? 1 : each < 8 ? static_cast<int>(each) : 8;
+    }
+    const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + span - 1) / span : 0);
     if (blocks > 0) {
         LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch",
                     job.heads, shape->seq_len);
-        const auto kernel = shape->head_size == 64 ? (job.tiles > 1 ? &finish_kernel<64, true> : &finish_kernel<64, false>)
-                                                   : (job.tiles > 1 ? &finish_kernel<128, true> : &finish_kernel<128, false>);
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, merges, mass_rounds);
+        const auto kernel = shape->head_size == 64 ? (kept ? &finish_kernel<64, true> : &finish_kernel<64, false>)
+                                                   : (kept ? &finish_kernel<128, true> : &finish_kernel<128, false>);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, merges, span);
         LPP_CHECK_LAUNCH("finish_kernel");
     }
     return LPP_OK;

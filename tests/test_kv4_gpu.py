@@ -266,6 +266,19 @@ def test_long_context(lib, heads, kv, hs, length):
     check_attention(got, got_mass, cache, 0, q, [length - 1], mass)
 
 
+@pytest.mark.parametrize("heads,kv,hs,n_q,lengths", [(16, 1, 64, 1, [4001]), (8, 2, 64, 1, [20011, 33]), (12, 1, 128, 1, [12001]), (4, 1, 64, 4, [3001, 900, 2])])
+def test_account_of_long_contexts(lib, heads, kv, hs, n_q, lengths):
+    """So many scores for each position that they are made again from K rather than kept."""
+    rng = np.random.default_rng(lengths[0])
+    room = lengths[0] + 2
+    cache = random_cache(rng, 1, len(lengths), kv, room, hs)
+    q = rng.standard_normal((len(lengths), n_q, heads, hs)).astype(F)
+    mass = rng.random((1, len(lengths), kv, room)).astype(F)
+    starts = [n - n_q for n in lengths]
+    got, got_mass = attend(lib, DB.from_numpy(cache.buffer), cache, 0, q, starts, mass)
+    check_attention(got, got_mass, cache, 0, q, starts, mass)
+
+
 def test_more_sequences_than_compute_units(lib):
     """Work enough without splitting anything."""
     rng = np.random.default_rng(77)
