@@ -103,8 +103,9 @@ __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& 
     return __builtin_amdgcn_readlane(rows, at);
 }
 
+// (wavefronts to a SIMD: registers for three where binary16 and heads of 64 need no more, two else)
 template <typename T, int kHs, int kR, int kP, int kStepRows>
-__global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) {
+__global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) void prompt_kernel(PromptJob job) {
     typedef Shape<kHs, kR, kP, kStepRows> S;
     constexpr bool kLo = sizeof(T) == 4;  // heads and remainders
     constexpr int kDTiles = kHs / 32, kKSteps = kHs / 16, kStep = S::kStep, kRowBytes = S::kRowBytes, kPieces = S::kPieces;
@@ -317,7 +318,7 @@ __global__ __launch_bounds__(64 * kR * kP, 2) void prompt_kernel(PromptJob job) 
                     step_sum = __builtin_amdgcn_fdot2(h, half2_t{static_cast<half_t>(1.0f), static_cast<half_t>(1.0f)}, step_sum, false);
                 }
             }
-if (kPartly && odd) {
+            if (kPartly && odd) {
                 // (uniform) A weight of zero would not keep it out.  One token after the other, with the rows behind it cleared; a lane's output is
                 // its own token's.
                 for (int token = 0; token < tokens_per_wave; ++token) {
@@ -453,15 +454,16 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
 // Which shape: the fewer tiles of 32 rows there are for each compute unit, the more wavefronts share a walk.  us, one prompt, 1 x 4 / 2 x 2 /
 // 4 x 1, 32 heads of 64 on 8, fp32: 256 rows (one tile a compute unit) 6.3 / 7.9 / 10.3; 512 9.3 / 11.7 / 14.8; 700 15.9 / 15.1 / 17.2; 1024 21.6 /
 // 20.7 / 24.1; 1500 38.6 / 33.3 / 34.5; 2048 59 / 56 / 49; 6000 - / 338 / 284.  32 heads of 128, binary16: 256 6.9 / 8.4 / 10.8; 400
-// 12.2 / 11.0 / 13.2; 1024 34 / 22 / 27; 1500 59 / 36 / 39; 2048 95 / 59 / 55; 6000 - / 381 / 321.  Steps of 4 x 1: 128 positions (heads of 64;
-// 64: 302 us at 6000 rows) or 64 (heads of 128; 32: 350).  (8 x 1: 326 and 331; the products of the next step formed between this
+// 12.2 / 11.0 / 13.2; 1024 34 / 22 / 27; 1500 59 / 36 / 39; 2048 95 / 59 / 55; 6000 - / 381 / 321.  Steps of 4 x 1: 128 positions (fp32, heads of 64;
+// 64: 302 us at 6000 rows) or 64 (heads of 128; 32: 350; binary16, heads of 64, where three workgroups fit on a compute unit so: 7 prompts of up to 1500
+// rows 49 us, 53 with 128).  (8 x 1: 326 and 331; the products of the next step formed between this
 // one's weights, a third stage, or other priorities for the products: no faster.)
 template <typename T, int kHs>
 lpp_status launch(const PromptJob& job, int n_seqs) {
     const long long tiles = (static_cast<long long>(job.n_tokens) * job.shared + 31) / 32 * job.n_kv_heads;  // of 32 rows
     if (tiles <= (kHs == 64 ? 2ll : 1ll) * compute_units()) return launch_as<T, kHs, 1, 4, 32>(job, n_seqs);
     if (tiles <= 6ll * compute_units()) return launch_as<T, kHs, 2, 2, 32>(job, n_seqs);
-    return launch_as<T, kHs, 4, 1, kHs == 64 ? 128 : 64>(job, n_seqs);
+    return launch_as<T, kHs, 4, 1, sizeof(T) == 4 && kHs == 64 ? 128 : 64>(job, n_seqs);
 }
 
 }  // namespace
