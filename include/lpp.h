@@ -471,10 +471,12 @@ enum { LPP_F32 = 0, LPP_F16 = 1 };
  * allowed.  NULL: one sequence of n_tokens rows (n_seqs is 1 then).  Rows of d_out that no sequence has are left as they
  * were.
  * q and out: [n_tokens][n_heads * head_size] of `type`; k and v: binary16 [n_tokens][n_kv_heads * head_size], what the
- * caches hold; the strides are the elements from one row to the next, kv_stride at most 2^24.  Rows start at multiples of 16 bytes.  d_out must
- * not overlap the inputs.  LPP_F32: queries and weights enter the products as binary16 head and remainder, as in
- * LPP_PREFILL_EXACT; LPP_F16: the weights are rounded to binary16 where V is weighted, sums are fp32, the output is rounded
- * once.  What K and V rows hold that a row does not attend to does not reach it, infinities and NaN included. */
+ * caches hold; the strides are the elements from one row to the next, kv_stride at most 2^24.  Rows start at multiples of
+ * 16 bytes.  d_out must not overlap the inputs.  LPP_F32: queries and weights enter the products as binary16 head and
+ * remainder, as in LPP_PREFILL_EXACT (a query beyond +-65504 gives NaN); LPP_F16: the weights are rounded to binary16 where V is weighted, sums are
+ * fp32, the output is rounded once.  What K and V rows hold that a row does not attend to does not reach it, infinities
+ * and NaN included; an infinity among the V values it does attend to gives an infinity or NaN.  The same inputs give the
+ * same bits. */
 lpp_status lpp_prompt_attention(void *d_out, const void *d_q, const lpp_half *d_k, const lpp_half *d_v, int type,
                                 const int *d_offsets, int n_seqs, int n_tokens, int n_heads, int n_kv_heads,
                                 int head_size, int q_stride, int kv_stride, int out_stride);
@@ -509,24 +511,26 @@ lpp_status lpp_kv4_load(lpp_half *d_k, lpp_half *d_v, const void *d_cache, const
 
 /* Attention of n_q new rows a sequence over one layer of the cache, which holds them already: row j attends to positions
  * 0 .. d_starts[s] + j, with the d_starts that the store was given (cut to the positions there are; a row that attends to
- * none gives zeros).  q and out: fp32 [n_seqs][n_q][n_heads * head_size], 16-byte aligned, not overlapping.  n_q = 1 is a
- * decode step.
+ * none gives zeros).  q and out: fp32 [n_seqs][n_q][n_heads * head_size], 16-byte aligned, not overlapping, a query beyond
+ * +-65504 gives NaN.  n_q = 1 is a decode step.
  * d_mass (may be NULL): fp32 [n_layers][n_seqs][n_kv_heads][seq_len]; to every position is added the weight it got, summed
  * over the rows and the query heads of its KV head.  Set it to zero when a sequence begins.
- * d_workspace: lpp_kv4_attention_workspace() bytes, 16-byte aligned; it need not be set to anything, and calls that may run
- * at the same time need one each.  The same inputs give the same bits. */
+ * d_workspace: lpp_kv4_attention_workspace() bytes, 16-byte aligned, apart from all else; it need not be set to anything,
+ * and calls that may run at the same time need one each.  The bytes grow with seq_len, n_heads and n_q, not with n_layers: one workspace
+ * serves all layers.  The same inputs give the same bits. */
 lpp_status lpp_kv4_attention_workspace(const lpp_kv4_shape *shape, int n_heads, int n_q, size_t *bytes);
 lpp_status lpp_kv4_attention(float *d_out, const float *d_q, const void *d_cache, const lpp_kv4_shape *shape, int layer,
                              int n_heads, int n_q, const int *d_starts, float *d_mass, void *d_workspace,
                              size_t workspace_bytes);
 
-/* One layer of a cache reduced to `keep` positions of every (sequence, KV head), into a layer of another cache, whose buffer must not overlap the first's: with n the sequence's
- * d_lengths (cut to 0 .. seq_len), all positions if n <= keep; else the last `recent` and, of the others, the keep - recent whose d_mass is
- * largest (equal ones: the lower position; NaN counts as largest), in the order they had.  Their rows go to positions
- * 0 .. of d_dst, their mass to d_dst_mass, whose further positions up to dst->seq_len are set to zero; rows behind the
- * kept ones stay as they were.  d_dst_lengths[s] = min(n, keep).  d_kept: [n_seqs][n_kv_heads][keep], the position each kept row
- * had, -1 behind them.  The shapes differ in n_layers and seq_len at most; 0 <= recent <= keep <= dst->seq_len.  d_dst_lengths must
- * not be d_lengths, nor d_dst_mass d_mass: the lengths are the same for every layer, and the next layer's call reads them again. */
+/* One layer of a cache reduced to `keep` positions of every (sequence, KV head), into a layer of another cache, whose
+ * buffer must not overlap the first's: with n the sequence's d_lengths (cut to 0 .. seq_len), all positions if n <= keep;
+ * else the last `recent` and, of the others, the keep - recent whose d_mass is largest (equal ones: the lower position;
+ * NaN counts as largest), in the order they had.  Their rows go to positions 0 .. of d_dst, their mass to d_dst_mass,
+ * whose further positions up to dst->seq_len are set to zero; rows behind the kept ones stay as they were.
+ * d_dst_lengths[s] = min(n, keep).  d_kept: [n_seqs][n_kv_heads][keep], the position each kept row had, -1 behind them.
+ * The shapes differ in n_layers and seq_len at most; 0 <= recent <= keep <= dst->seq_len.  d_dst_lengths must not be
+ * d_lengths, nor d_dst_mass d_mass: the lengths are the same for every layer, and the next layer's call reads them again. */
 lpp_status lpp_kv4_evict(void *d_dst, const lpp_kv4_shape *dst, int dst_layer, float *d_dst_mass, int *d_dst_lengths,
                          int *d_kept, const void *d_src, const lpp_kv4_shape *src, int src_layer, const float *d_mass,
                          const int *d_lengths, int keep, int recent);

@@ -57,6 +57,17 @@ inline bool ranges_overlap(const void* a, size_t a_bytes, const void* b, size_t 
     return x < y + b_bytes && y < x + a_bytes;
 }
 
+// A kernel's LDS need, told to the runtime once per device (the attribute belongs to the device's copy of the kernel).
+inline lpp_status tell_lds(const void* kernel, int bytes, bool (&told)[64]) {
+    int device = 0;
+    LPP_HIP(hipGetDevice(&device));
+    if (device < 0 || device >= 64 || !told[device]) {
+        LPP_HIP(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (device >= 0 && device < 64) told[device] = true;
+    }
+    return LPP_OK;
+}
+
 namespace dev {
 
 // The eight binary16 numbers that a word of codes stands for.  A code in the last bits of a half whose exponent is that of 1024 is

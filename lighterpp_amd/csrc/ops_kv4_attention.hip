@@ -675,14 +675,9 @@ template <int kHs, int kWaves>
 lpp_status launch_attend(const AttendJob& job, dim3 grid) {
     constexpr int kLds = kWaves * ((kRows * (kHs + 4) + 2 * kRows) * 4 + ScaleRows<kHs>::kLdsBytes) + Queries<kHs>::kLdsBytes;
     const auto kernel = &attend_kernel<kHs, kWaves>;
-    if constexpr (kLds > 64 * 1024) {  // told to the runtime once per device
+    if constexpr (kLds > 64 * 1024) {
         static bool sized[64] = {};
-        int device = 0;
-        LPP_HIP(hipGetDevice(&device));
-        if (device < 0 || device >= 64 || !sized[device]) {
-            LPP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-            if (device >= 0 && device < 64) sized[device] = true;
-        }
+        LPP_TRY(tell_lds(reinterpret_cast<const void*>(kernel), kLds, sized));
     }
     hipLaunchKernelGGL(kernel, grid, dim3(kWave * kWaves), kLds, stream(), job);
     LPP_CHECK_LAUNCH("attend_kernel");
@@ -731,6 +726,10 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     LPP_REQUIRE(!ranges_overlap(d_workspace, need, d_q, rows_bytes) && !ranges_overlap(d_workspace, need, d_out, rows_bytes) &&
                     !ranges_overlap(d_workspace, need, d_cache, kv4_bytes(*shape)),
                 "lpp_kv4_attention: the workspace overlaps q, out or the cache");
+    const size_t mass_bytes = d_mass != nullptr ? kv4_layer_rows(*shape) * shape->n_layers * 4 : 0;
+    LPP_REQUIRE(mass_bytes == 0 || (!ranges_overlap(d_mass, mass_bytes, d_workspace, need) && !ranges_overlap(d_mass, mass_bytes, d_q, rows_bytes) &&
+                                    !ranges_overlap(d_mass, mass_bytes, d_out, rows_bytes) && !ranges_overlap(d_mass, mass_bytes, d_cache, kv4_bytes(*shape))),
+                "lpp_kv4_attention: d_mass overlaps the workspace, q, out or the cache");
     AttendJob job;
     job.out = d_out;
     job.q = d_q;

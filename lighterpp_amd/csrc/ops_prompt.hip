@@ -432,14 +432,9 @@ template <typename T, int kHs, int kR, int kP, int kStepRows>
 lpp_status launch_as(const PromptJob& job, int n_seqs) {
     constexpr int kLds = Shape<kHs, kR, kP, kStepRows>::kLdsBytes;
     const auto kernel = &prompt_kernel<T, kHs, kR, kP, kStepRows>;
-    if constexpr (kLds > 64 * 1024) {  // told to the runtime once per device
+    if constexpr (kLds > 64 * 1024) {
         static bool sized[64] = {};
-        int device = 0;
-        LPP_HIP(hipGetDevice(&device));
-        if (device < 0 || device >= 64 || !sized[device]) {
-            LPP_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
-            if (device >= 0 && device < 64) sized[device] = true;
-        }
+        LPP_TRY(tell_lds(reinterpret_cast<const void*>(kernel), kLds, sized));
     }
     // (as many tiles as sequences of any lengths can have)
     const int tokens = kR * (32 / job.shared);

@@ -82,8 +82,8 @@ def test_attention_refused(lib):
     need = C.c_size_t()
     capi.check(lib.lpp_kv4_attention_workspace(s, 8, 2, C.byref(need)))
     assert need.value > 0
-    call = lambda out=P, q=2 * P, cache=3 * P, layer=0, heads=8, n_q=2, starts=P, work=4 * P, size=need.value: \
-        lib.lpp_kv4_attention(out, q, cache, s, layer, heads, n_q, starts, None, work, size)  # noqa: E731
+    call = lambda out=P, q=2 * P, cache=3 * P, layer=0, heads=8, n_q=2, starts=P, work=4 * P, size=need.value, mass=None: \
+        lib.lpp_kv4_attention(out, q, cache, s, layer, heads, n_q, starts, mass, work, size)  # noqa: E731
     refused(lib, call(out=None), b"null pointer")
     refused(lib, call(q=None), b"null pointer")
     refused(lib, call(starts=None), b"null pointer")
@@ -100,6 +100,8 @@ def test_attention_refused(lib):
     refused(lib, call(work=2 * P + 64), b"workspace")
     refused(lib, call(work=P - 64), b"workspace")
     refused(lib, call(work=3 * P + 64), b"workspace")
+    for base in (P, 2 * P, 3 * P, 4 * P):
+        refused(lib, call(mass=base + 64), b"d_mass overlaps")
     for name in ("out", "q", "work"):
         refused(lib, call(**{name: 5 * P + 4}), b"16 bytes")
     refused(lib, lib.lpp_kv4_attention_workspace(s, 8, 2, None), b"null output")

@@ -1,11 +1,14 @@
 """lpp_prompt_attention against 64 bits: ragged and empty sequences, every number of query heads to a KV head, both types, strides, rows that
 belong to no sequence, and what K and V hold outside a row's own positions."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import kv4_oracle as ko
 from lighterpp_amd import capi
 from lighterpp_amd.capi import DeviceBuffer as DB
+from test_kv4_gpu import Hip
 
 pytestmark = pytest.mark.gpu
 F, H = np.float32, np.float16
@@ -189,3 +192,44 @@ def test_rows_far_apart(lib):
     want, _, tol = ko.attend_tolerance(q[keep], k.transpose(1, 0, 2), v.transpose(1, 0, 2), ends, binary16=True)
     got = np.stack([dout.to_numpy(H, heads * hs, r * stride * 2).reshape(heads, hs) for r in keep]).astype(np.float64)
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("heads,kv,hs,typ", [(8, 2, 64, F), (8, 8, 64, H), (4, 1, 128, F), (8, 2, 128, H)])
+def test_captured_in_a_graph(lib, heads, kv, hs, typ):
+    """Captured once, replayed with other rows and offsets in place and eager calls of the library between: the bits of the eager calls."""
+    hip = Hip()
+    rng = np.random.default_rng(heads + hs)
+    rows = 900
+    size = 4 if typ is F else 2
+    q, k, v, offsets = DB(rows * heads * hs * size), DB(rows * kv * hs * 2), DB(rows * kv * hs * 2), DB(16)
+    out = [DB.from_numpy(np.zeros(rows * heads * hs, typ)) for _ in range(2)]
+    side, graph, ready = hip.stream(), C.c_void_p(), C.c_void_p()
+
+    def call(into):
+        capi.check(lib.lpp_prompt_attention(into.ptr, q.ptr, k.ptr, v.ptr, capi.F32 if typ is F else capi.F16, offsets.ptr, 3, rows, heads, kv, hs,
+                                            heads * hs, kv * hs, heads * hs))
+
+    capi.synchronize()
+    try:
+        capi.check(lib.lpp_set_stream(side))
+        hip("hipStreamBeginCapture", side, 2)
+        try:
+            call(out[0])
+        finally:
+            hip("hipStreamEndCapture", side, C.byref(graph))
+        capi.check(lib.lpp_set_stream(None))
+        hip("hipGraphInstantiate", C.byref(ready), graph, None, None, C.c_size_t(0))
+        for at in ([0, 1, 300, 900], [0, 0, 0, 0], [5, 400, 401, 899], [0, 900, 900, 900]):
+            for buffer, n, t in ((q, heads, typ), (k, kv, H), (v, kv, H)):
+                buffer.upload(rng.standard_normal((rows, n * hs)).astype(t))
+            offsets.upload(np.array(at, np.int32))
+            call(out[1])
+            capi.synchronize()
+            hip("hipGraphLaunch", ready, side)
+            hip("hipStreamSynchronize", side)
+            assert np.array_equal(out[0].to_numpy(np.uint8), out[1].to_numpy(np.uint8)), at
+        hip("hipGraphExecDestroy", ready)
+        hip("hipGraphDestroy", graph)
+    finally:
+        capi.check(lib.lpp_set_stream(None))
+        hip("hipStreamDestroy", side)
