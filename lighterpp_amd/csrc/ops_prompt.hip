@@ -1,5 +1,21 @@
 // ops_prompt.hip -- lpp_prompt_attention: causal attention of whole prompts,
 // packed one behind the other.
+//
+// out[t] = sum_p w(t, p) v[p] / sum_p w(t, p) with w(t, p) = 2^(scale q[t] . k[p] - top(t)), over the positions p <= t of t's sequence, scale =
+// log2(e) / sqrt(head_size).  One walk over the positions: `top` is a score of the row so far, moved (and sum and output rescaled) only when a score
+// passes it by more than kSlack; any value near the maximum would do, since it cancels.
+//
+// Both products run on the matrix cores, 32 positions x 32 query rows at a time: scores = K Q^T, whose result has a query row to a
+// lane and its positions in that lane's registers, as the second product, V^T W^T, wants its second operand; so weights never leave
+// registers, and maximum and sum of a row are two lanes' business.  The order in which the first product's rows come out is made good by the order in which
+// transposing reads take V rows from LDS.  fp32: queries and weights enter as binary16 head and remainder, twice the products.
+//
+// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 576 to 620 us, 890 to 950 TFLOP/s, where a matrix product
+// of 8192^3 reaches 1186; LDS is read for 63 % of the time, the matrix cores are busy 40 %, vector ALUs 46 %.  Weights without exponentials, no maximum,
+// or no multiplication by the scale gain 0 to 10 %; two query tiles to a wavefront, for half the reads of LDS, are slower (half the
+// wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of 128 do not fit the registers).  Several pages (7 of up to 1500 rows, 32
+// heads of 64 on 8, fp32): 114 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us, the time of the requests one
+// after the other: offsets, rows, and the write.
 #include <type_traits>
 
 #include "kv4.hpp"
@@ -204,7 +220,7 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
     for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-    constexpr float kSlack = 6.0f;
+    constexpr float kSlack = 6.0f;  // weights stay below 2^6: their sums are far from fp32's limits, and in binary16 from its largest
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
     float top = 0.0f, lsum = 0.0f;  // (the sum over this lane's own positions)
     bool seen = false;              // the row has attended to something: top is a score
