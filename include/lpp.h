@@ -482,7 +482,7 @@ lpp_status lpp_prompt_attention(void *d_out, const void *d_q, const lpp_half *d_
                                 int head_size, int q_stride, int kv_stride, int out_stride);
 
 /* A cache of 4 bits.  A group is 32 values of a K or V row.  Its lowest value l is rounded to binary16, its scale c is
- * (highest - lowest) / 15 in fp32, rounded to binary16; a value's code is the integer nearest to (value - l) / c (ties to even,
+ * (highest - lowest) * (1 / 15) in fp32, rounded to binary16; a value's code is the integer nearest to (value - l) / c (ties to even,
  * 0 if c is 0), cut to 0 .. 15, and stands for l + code * c, rounded once to binary16.  A group with a value that is
  * not finite or beyond +-32768 stands for NaN throughout, so that an overflow shows.  5 bits a value in all.
  * One buffer of lpp_kv4_bytes() bytes, 16-byte aligned, in four parts: codes of K, codes of V, scales of K, scales of V, each

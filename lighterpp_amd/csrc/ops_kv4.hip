@@ -57,15 +57,11 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, flo
     return word;
 }
 
-// r / 15 rounded to nearest: the product with the rounded reciprocal, and once more with what it leaves (equal to the quotient
-// for every mantissa; results that a binary16 rounds to 0 aside).  The result is hidden from the compiler, which would otherwise
-// form the last step and its rounding to binary16 in one instruction, with one rounding.
+// The product is hidden from the compiler, which would otherwise form it and its rounding to binary16 in one instruction, with one rounding.
 __device__ __forceinline__ float fifteenth(float r) {
-    constexpr float kInverse = 1.0f / 15.0f;
-    const float q = r * kInverse;
-    float quotient = fmaf(fmaf(q, -15.0f, r), kInverse, q);
-    asm("" : "+v"(quotient));
-    return quotient;
+    float product = r * (1.0f / 15.0f);
+    asm("" : "+v"(product));
+    return product;
 }
 
 // One wavefront per row, K and V; a lane has a word's eight values, two words of each at a time.  The first values are requested along with the

@@ -14,7 +14,7 @@ def quantise(x):
     bad = ~(np.abs(g) <= 32768).all(-1)
     g = np.where(bad[..., None], F32(0), g)
     low, high = g.min(-1), g.max(-1)
-    scale = ((high - low) / F32(15)).astype(F16)
+    scale = ((high - low) * (F32(1) / F32(15))).astype(F16)
     low = low.astype(F16)
     with np.errstate(divide="ignore", invalid="ignore"):
         t = np.rint((g.astype(F64) - low.astype(F64)[..., None]) / scale.astype(F64)[..., None])
