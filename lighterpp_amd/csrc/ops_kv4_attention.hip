@@ -60,6 +60,10 @@ struct AttendJob {
     }
 };
 
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 __device__ __forceinline__ float rows_max(float v) {
     const unsigned u = __float_as_uint(v);
     const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -439,8 +443,8 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     }
 }
 
-// What is left once every share has been walked: blocks before `merges` (where there are shares to merge) merge a row each, the others add up
-// the weights of the positions.
+// What is left once every share has been walked: the first blocks, `accounts` of them, add up the weights of the positions, the others (where there
+// are shares to merge) merge a row with each wavefront.
 constexpr int kFinishWaves = 4, kFinishThreads = kWave * kFinishWaves;
 
 // Maximum and 1 / sum of a tile's rows, each in the lanes that have its column: the shares' in four parts, which meet across those lanes.
@@ -473,11 +477,9 @@ struct Sums {
 
 // kKept: the account is made from the scores that the shares have kept; else from K again.
 template <int kHs, bool kKept>
-__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int merges, int span) {
-    constexpr int kFours = kHs / 4, kSlices = kFinishThreads / kFours, kPieces = 4, kOfWave = 16 * kPieces;
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, int accounts, int span) {
+    constexpr int kFours = kHs / 4, kSlices = kWave / kFours, kPieces = 4, kOfWave = 16 * kPieces;
     constexpr int kQueryBytes = Queries<kHs>::kLdsBytes > 0 ? Queries<kHs>::kLdsBytes : 16;
-    __shared__ float weights[kMaxSplits];
-    __shared__ __align__(16) float partial[kSlices][kHs];
     __shared__ __align__(16) char scale_lds[kFinishWaves][ScaleRows<kHs>::kLdsBytes];
     __shared__ __align__(16) char q_lds[kFinishWaves][kQueryBytes];
     __shared__ float of_waves[kFinishWaves][kOfWave];
@@ -486,50 +488,58 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
     const int kvh = head % job.n_kv_heads, s = head / job.n_kv_heads, start = job.start_of(s), tokens = job.tokens();
     const int all_end = job.end_of(start, job.n_q - 1);
     const int active = job.shares_of(all_end);
-    if (block < merges) {
+    if (block >= accounts) {
+        // A wavefront to a row: its lanes have four values each of every kSlices-th share.
         if (active == 1) return;
-        const int tile = block / job.rows, row = block % job.rows;
+        const int index = (block - accounts) * kFinishWaves + wave;
+        if (index >= job.tiles * job.rows) return;
+        const int tile = index / job.rows, row = index % job.rows;
         const Column its(job, tile, row);
         if (!its.valid) return;
         const size_t slot = (static_cast<size_t>(head) * job.tiles + tile) * job.splits;
-        // (the shares' outputs are requested along with their weights; a share that the row does not attend to has left none)
-        const int slice = static_cast<int>(threadIdx.x) / kFours, four = static_cast<int>(threadIdx.x) % kFours;
-        constexpr int kEach = kMaxSplits / kSlices;
-        floatx4 a[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (kSlices * i >= active) break;  // (uniform)
-            const int at = min(slice + kSlices * i, active - 1);
-            a[i] = *reinterpret_cast<const floatx4*>(job.partials + ((slot + at) * job.rows + row) * kHs + 4 * four);
-        }
+        const int slice = lane / kFours, four = lane % kFours;
         const float2 st = lane < active ? job.stats[(slot + lane) * job.rows + row] : make_float2(-INFINITY, 0.0f);
-        float top = wave_max(st.x);
-        if (top == -INFINITY) top = 0.0f;
-        const float weight = __builtin_amdgcn_exp2f(st.x - top);
-        const float total = wave_sum(st.y * weight);
-        if (wave == 0) weights[lane] = st.x == -INFINITY && st.y == 0.0f ? -1.0f : weight;
-        __syncthreads();
+        const float* from = job.partials + (slot * job.rows + row) * kHs + 4 * four;
         floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        float weight = 0.0f, total = 0.0f;
+        // (the shares' outputs are requested along with their sums, kAtOnce rounds of them; a share that the row does not attend to has left none)
+        constexpr int kAtOnce = 8;
+        for (int i0 = 0; i0 < active; i0 += kAtOnce * kSlices) {
+            floatx4 a[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (kSlices * i >= active) break;
-            const int at = slice + kSlices * i;
-            const float w = weights[at];
-            if (at < active && w >= 0.0f)
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (i0 + i * kSlices >= active) break;  // (uniform)
+                a[i] = *reinterpret_cast<const floatx4*>(from + static_cast<size_t>(min(i0 + i * kSlices + slice, active - 1)) * job.rows * kHs);
+            }
+            if (i0 == 0) {
+                float top = wave_max(st.x);
+                if (top == -INFINITY) top = 0.0f;
+                weight = __builtin_amdgcn_exp2f(st.x - top);
+                total = wave_sum(st.y * weight);
+                if (st.x == -INFINITY && st.y == 0.0f) weight = -1.0f;  // (lanes without a share too)
+            }
+            float w[kAtOnce];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[i][u], w, sum[u]);
+            for (int i = 0; i < kAtOnce; ++i) w[i] = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (i0 + i * kSlices + slice), __float_as_int(weight)));
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (i0 + i * kSlices >= active) break;
+                if (w[i] >= 0.0f)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) sum[u] = fmaf(a[i][u], w[i], sum[u]);
+            }
         }
-        *reinterpret_cast<floatx4*>(&partial[slice][4 * four]) = sum;
-        __syncthreads();
-        if (threadIdx.x < kHs) {
-            float v = 0.0f;
+        const bool any = job.end_of(start, its.token) > 0;
+        const float inverse = 1.0f / total;
 #pragma unroll
-            for (int i = 0; i < kSlices; ++i) v += partial[i][threadIdx.x];
-            job.out[its.at(job, s, kvh) * kHs + threadIdx.x] = job.end_of(start, its.token) > 0 ? v / total : 0.0f;
+        for (int u = 0; u < 4; ++u) {
+            sum[u] = kSlices == 4 ? rows_sum(sum[u]) : halves_sum(sum[u]);
+            sum[u] = any ? sum[u] * inverse : 0.0f;
         }
+        if (slice == 0) *reinterpret_cast<floatx4*>(job.out + its.at(job, s, kvh) * kHs + 4 * four) = sum;
         return;
     }
-    const int p_first = (block - merges) * span;
+    const int p_first = block * span;
     if (p_first >= all_end) return;
     float* mass = job.mass + (static_cast<size_t>(s) * job.n_kv_heads + kvh) * job.seq_len;
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
@@ -780,7 +790,7 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
         LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
     else
         LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
-    const int merges = job.splits > 1 ? job.tiles * job.rows : 0;
+    const int merges = job.splits > 1 ? (job.tiles * job.rows + kFinishWaves - 1) / kFinishWaves : 0;
     // The positions of one of the account's blocks.  From kept scores of one tile: as many rounds of 1024, up to 8, as leave four blocks to a compute
     // unit.
     const bool kept = job.scores != nullptr;
@@ -789,13 +799,13 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
         const long long each = (static_cast<long long>(shape->seq_len) + span - 1) / span * job.heads / (4 * compute_units());
         span *= each < 1 ? 1 : each < 8 ? static_cast<int>(each) : 8;
     }
-    const int blocks = merges + (d_mass != nullptr ? (shape->seq_len + span - 1) / span : 0);
+    const int accounts = d_mass != nullptr ? (shape->seq_len + span - 1) / span : 0, blocks = merges + accounts;
     if (blocks > 0) {
         LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch",
                     job.heads, shape->seq_len);
         const auto kernel = shape->head_size == 64 ? (kept ? &finish_kernel<64, true> : &finish_kernel<64, false>)
                                                    : (kept ? &finish_kernel<128, true> : &finish_kernel<128, false>);
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, merges, span);
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, accounts, span);
         LPP_CHECK_LAUNCH("finish_kernel");
     }
     return LPP_OK;
