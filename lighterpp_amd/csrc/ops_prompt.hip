@@ -11,7 +11,7 @@
 // transposing reads take V rows from LDS.  fp32: queries and weights enter as binary16 head and remainder, twice the products.
 //
 // What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 576 to 620 us, 890 to 950 TFLOP/s, where a matrix product
-// of 8192^3 reaches 1186; LDS is read for 63 % of the time, the matrix cores are busy 40 %, vector ALUs 46 %.  Weights without exponentials, no maximum,
+// of 8192^3 reaches 1186; the matrix cores are busy 44 % of the cycles, vector ALUs 49 %, LDS 22 %.  Weights without exponentials, no maximum,
 // or no multiplication by the scale gain 0 to 10 %; two query tiles to a wavefront, for half the reads of LDS, are slower (half the
 // wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of 128 do not fit the registers).  Several pages (7 of up to 1500 rows, 32
 // heads of 64 on 8, fp32): 114 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us, the time of the requests one
