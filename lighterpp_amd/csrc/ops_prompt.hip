@@ -227,6 +227,11 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
     float minus_one = -1.0f;
     asm("" : "+v"(minus_one));
 
+    // (Q has landed: the loops, whose own requests are under way, do not wait for it)
+    if constexpr (!kLo)
+#pragma unroll
+        for (int s = 0; s < kKSteps; ++s) asm volatile("" : "+v"(qh[s]));
+
     // where this lane reads its fragments of a tile: K row r, pieces 2 s + g; V rows 4 g + (lane % 16) / 4 of the first
     // sixteen, dimensions 32 dt + 16 (lane / 16 % 2) + 4 (lane % 4) ..
     int k_at[kKSteps], v_at[kDTiles];
@@ -361,22 +366,28 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
         }
         lsum += step_sum;
     };
-    for (int turn = 0; turn < turns; ++turn) {
-        const int p0 = (turn * kP + wp) * kStep;
+    auto rows_of = [&](int turn) -> const char* {  // K rows of a turn's step, V rows behind them; the next ones requested
         // (the step's rows have landed, and nobody reads the stage the next requests go to any more)
         wait_requests<0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if constexpr (kR > 1) __syncthreads();
         if (turn + 1 < turns) request(turn + 1);
-        const char* keys = stages + (turn % S::kStages) * S::kStageBytes;
-        const char* values = keys + S::kHalfBytes;
-        if (p0 + kStep <= t0 + 1) {  // (uniform)
-            walk(std::false_type{}, std::integral_constant<int, kTiles>{}, p0, keys, values);
-        } else {
+        return stages + (turn % S::kStages) * S::kStageBytes;
+    };
+    // First the steps that every row of the wavefront attends to, then those that some do not.  (Two loops: with a branch in one, every step
+    // would copy `o` between the registers that its two ways have it in.)
+    const int whole_steps = (t0 + 1) / kStep, whole_turns = min(turns, (max(whole_steps - wp, 0) + kP - 1) / kP);
+    int turn = 0;
+    for (; turn < whole_turns; ++turn) {
+        const char* keys = rows_of(turn);
+        walk(std::false_type{}, std::integral_constant<int, kTiles>{}, (turn * kP + wp) * kStep, keys, keys + S::kHalfBytes);
+    }
+    for (; turn < turns; ++turn) {
+        const char* keys = rows_of(turn);
+        const int p0 = (turn * kP + wp) * kStep;
 #pragma unroll 1
-            for (int t = 0; t < kTiles && p0 + 32 * t < wave_limit; ++t)
-                walk(std::true_type{}, std::integral_constant<int, 1>{}, p0 + 32 * t, keys + t * 32 * kRowBytes, values + t * 32 * kRowBytes);
-        }
+        for (int t = 0; t < kTiles && p0 + 32 * t < wave_limit; ++t)
+            walk(std::true_type{}, std::integral_constant<int, 1>{}, p0 + 32 * t, keys + t * 32 * kRowBytes, keys + S::kHalfBytes + t * 32 * kRowBytes);
     }
     lsum = halves_sum(lsum);
     T* out_row = static_cast<T*>(job.out) + static_cast<size_t>(first_row + tok_c) * job.out_stride + (kvh * job.shared + my_head) * kHs + 4 * g;
@@ -466,15 +477,15 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
 // 4 x 1, 32 heads of 64 on 8, fp32: 256 rows (one tile a compute unit) 6.3 / 7.9 / 10.3; 512 9.3 / 11.7 / 14.8; 700 15.9 / 15.1 / 17.2; 1024 21.6 /
 // 20.7 / 24.1; 1500 38.6 / 33.3 / 34.5; 2048 59 / 56 / 49; 6000 - / 338 / 284.  32 heads of 128, binary16: 256 6.9 / 8.4 / 10.8; 400
 // 12.2 / 11.0 / 13.2; 1024 34 / 22 / 27; 1500 59 / 36 / 39; 2048 95 / 59 / 55; 6000 - / 381 / 321.  Steps of 4 x 1: 128 positions (fp32, heads of 64;
-// 64: 302 us at 6000 rows) or 64 (heads of 128; 32: 350; binary16, heads of 64, where three workgroups fit on a compute unit so: 7 prompts of up to 1500
-// rows 49 us, 53 with 128).  (8 x 1: 326 and 331; the products of the next step formed between this
+// 64: 302 us at 6000 rows), 64 (binary16, heads of 128; 32: 350; heads of 64, where three workgroups fit on a compute unit so: 7 prompts of up to
+// 1500 rows 45 us, 49 with 128) or 32 (fp32, heads of 128, where 64 spill: the same prompts 122 us for 131).  (8 x 1: 326 and 331; the products of the next step formed between this
 // one's weights, a third stage, or other priorities for the products: no faster.)
 template <typename T, int kHs>
 lpp_status launch(const PromptJob& job, int n_seqs) {
     const long long tiles = (static_cast<long long>(job.n_tokens) * job.shared + 31) / 32 * job.n_kv_heads;  // of 32 rows
     if (tiles <= (kHs == 64 ? 2ll : 1ll) * compute_units()) return launch_as<T, kHs, 1, 4, 32>(job, n_seqs);
     if (tiles <= 6ll * compute_units()) return launch_as<T, kHs, 2, 2, 32>(job, n_seqs);
-    return launch_as<T, kHs, 4, 1, sizeof(T) == 4 && kHs == 64 ? 128 : 64>(job, n_seqs);
+    return launch_as<T, kHs, 4, 1, sizeof(T) == 2 ? 64 : kHs == 64 ? 128 : 32>(job, n_seqs);
 }
 
 }  // namespace
