@@ -263,6 +263,19 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
                 if constexpr (kLo) st[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, ql[s], st[t], 0, 0, 0);
             }
         }
+        if constexpr (!kPartly) {
+            // Six of K's fragments on their way before the first product, another with each product (left to the compiler, each is requested when the
+            // last one is used: 2048 rows, 32 heads of 128, binary16, 58 us for 54).
+            constexpr int kFragments = kTiles * kKSteps, kAhead = kFragments < 6 ? kFragments : 6, kProducts = kLo ? 2 : 1;
+            constexpr int kMatrix = 0x008, kLdsRead = 0x100;
+            __builtin_amdgcn_sched_group_barrier(kLdsRead, kAhead, 0);
+#pragma unroll
+            for (int i = 0; i < kFragments - kAhead; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kMatrix, kProducts, 0);
+                __builtin_amdgcn_sched_group_barrier(kLdsRead, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(kMatrix, kProducts * kAhead, 0);
+        }
         if constexpr (kPartly) {
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
