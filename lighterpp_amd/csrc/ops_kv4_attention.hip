@@ -222,7 +222,8 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         codes[w] = job.cache.codes[w] + head_rows * (kHs / 8);
         scales[w] = job.cache.scales[w] + head_rows * (kHs / kKv4Group);
     }
-    // K and V of a step travel while the step before is worked on, each requested as soon as its registers are free.
+    // K and V of a step travel while the step before is worked on, each requested as soon as its registers are free.  (Also behind the last
+    // step, whose requests are the last row's again: were they conditional, a wait for one would have to be a wait for all.)
     Piece<kHs> k[2], v[2];
     auto request = [&](Piece<kHs>(&to)[2], int which, int p0) {
 #pragma unroll
@@ -264,14 +265,13 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         for (int i = 0; i < kWords; ++i) v_to[i] = column * kRowBytes + 16 * ((kWords * part + i) ^ swizzle(column));
     }
 
-    // (after the step's requests, so that none of those waits for these stores)
+    // (stored behind the step's requests of K and V, so that those do not wait for the stores)
     const bool keeps = job.scores != nullptr && mine.valid;
     float* my_scores = job.scores + (static_cast<size_t>(head) * job.steps * job.rows + min(column, job.rows - 1)) * kStep + 4 * part;
     for (int p0 = first; p0 < end; p0 += stride) {
-        const bool more = p0 + stride < end;         // (uniform)
         const bool partly = p0 + kStep > first_end;   // (uniform) some row does not attend to the whole step
         pairs.put(pairs_lds);
-        if (more) request_pairs(p0 + stride);
+        request_pairs(p0 + stride);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             k[t].pair = ScaleRows<kHs>::get(pairs_lds, 16 * t + column, part);
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         }
         floatx4 st[2];
         q.template scores<2>(read, k, st);
-        if (more) request(k, 0, p0 + stride);
+        request(k, 0, p0 + stride);
         // V rows behind the tile's last position are zero: a weight of zero does not keep an infinity or NaN out.
         if (partly) {
 #pragma unroll
@@ -291,16 +291,16 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < kWords; ++i) *reinterpret_cast<half8_t*>(values + v_to[i] + 16 * t * kRowBytes) = v[t].values(read, i);
-        if (more) request(v, 1, p0 + stride);
+        request(v, 1, p0 + stride);
+        if (keeps) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) *reinterpret_cast<floatx4*>(my_scores + p0 * job.rows + 16 * t) = st[t];
+        }
         if (partly) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) st[t][e] = p0 + 16 * t + 4 * part + e < my_end ? st[t][e] : -INFINITY;
-        }
-        if (keeps) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t) *reinterpret_cast<floatx4*>(my_scores + p0 * job.rows + 16 * t) = st[t];
         }
         float step_top = -INFINITY;
 #pragma unroll
