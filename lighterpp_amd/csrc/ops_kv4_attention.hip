@@ -772,10 +772,10 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     const Split split = split_of(*shape, job.tiles);
     job.splits = split.splits;
     job.least = split.least;
-    // (a quarter more shares than run at once: they are of unequal length, and the last to begin are not the last to end.  us for 1 / 1.25 / 1.5 / 2
-    // times as many, heads of 128, ragged: 32 sequences of up to 8000 positions 62 / 59 / 56 / 58, 64 of 4000 60 / 58 / 58 / 59, 8 of 8000 28 / 28 / 31 / 31,
-    // 3 of 16000 24.7 / 23.1 / 22.2 / 25.0)
-    job.per_workgroup = static_cast<float>(shape->n_kv_heads) * job.tiles / (1.25f * split.workgroups);
+    // Of many heads a quarter more shares than run at once: they are of unequal length, and the last to begin are not the last to end.  us for 1 / 1.25 /
+    // 1.5 / 2 times as many, heads of 128, ragged: 32 sequences of up to 8000 positions 62 / 59 / 56 / 58, 64 of 4000 60 / 58 / 58 / 59; 32 of 4000 alike 43 / 41.  Of few
+    // heads no more than run at once: 4 sequences of 8000 alike 17 / 23.
+    job.per_workgroup = static_cast<float>(shape->n_kv_heads) * job.tiles / (split.waves == 4 ? 1.25f * split.workgroups : split.workgroups);
     job.per_shared = (65536u + job.shared - 1) / job.shared;
     const Workspace parts(*shape, n_q, job.shared, job.tiles, job.splits);
     job.rows = parts.rows;
