@@ -12,8 +12,8 @@
 // nothing else would have to be formed.  Queries and weights enter as binary16 head and remainder.  V goes through LDS, for transposing
 // reads.
 //
-// What bounds it: 32 sequences of up to 8000 positions, 32 heads of 128 on 8: 65 us (3.2 TB/s of the 160 bytes a position and KV head; reading alone
-// takes 47), and 10 for the account; the rest is instructions for the codes.  One sequence of 16001, heads of 64: 7.6 + 2.7 us, one of 500:
+// What bounds it: 32 sequences of up to 8000 positions, 32 heads of 128 on 8: 60 us with the scores kept for the account (3.4 TB/s of the 160 bytes a
+// position and KV head; reading alone takes 47), and 9 for it and the merge; the rest is instructions for the codes.  One sequence of 16001, heads of 64: 7.6 + 3 us, one of 500:
 // 6.5 us: the time of requests one after the other, a start and a merge.
 #include "kv4.hpp"
 
@@ -677,7 +677,7 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
 }
 
 // What the workspace holds.  Scores kept for the account are 4 bytes for every position and row; made from K again they cost its bytes and the
-// products (32 sequences of up to 8000 positions, 4 rows to a KV head of 128: 49 us more than without an account, and 14 so).  Not of several tiles, whose
+// products (32 sequences of up to 8000 positions, 4 rows to a KV head of 128: 49 us more than without an account, and 10 so).  Not of several tiles, whose
 // scores are many times a layer (16 rows of 32 heads, 4 sequences of up to 3000 positions, heads of 64: 27.5 us for 25.5), and only where
 // the workspace gets no larger than partial results of kMaxSplits shares would make it: up to 14000 positions with four rows to a KV head of 64,
 // 2000 with sixteen.
