@@ -451,43 +451,44 @@ lpp_status lpp_trace_token_all(lpp_model *m, int pos, unsigned long long *out, i
 /* E. Several prompts at once, and a key/value cache of 4 bits            */
 /* ===================================================================== */
 
-/* Beside section A's operators for one token and one binary16 cache (no counterpart in the reference).  The calls that
- * belong together: lpp_prompt_attention over prompts that arrived together; lpp_kv4_store of their K and V rows; then, a
- * token at a time, lpp_kv4_store and lpp_kv4_attention, which may count what every position is worth; and lpp_kv4_evict,
- * which reduces the cache to the positions worth most.  All pointers are device memory, every call is queued on the
- * library's stream and returns; nothing is allocated, and nothing is kept from one call for the next.  What the device
- * arrays of ints hold cannot be refused by the call: values outside their range are cut to it as written below, and no
- * access leaves the buffers.
+/* Beside section A's operators for one token and one binary16 cache (no counterpart in the reference).  The
+ * calls that belong together: lpp_prompt_attention over prompts that arrived together; lpp_kv4_store of their K
+ * and V rows; then, a token at a time, lpp_kv4_store and lpp_kv4_attention, which may count what every position
+ * is worth; and lpp_kv4_evict, which reduces the cache to the positions worth most.  All pointers are device
+ * memory, every call is queued on the library's stream and returns; nothing is allocated, and nothing is kept
+ * from one call for the next.  What the device arrays of ints hold cannot be refused by the call: values
+ * outside their range are cut to it as written below, and no access leaves the buffers.
  *
- * n_heads is a multiple of n_kv_heads, at most 16 query heads to a KV head; query head h uses KV head
- * h / (n_heads / n_kv_heads).  head_size is 64 or 128.  Scores are q . k / sqrt(head_size), as everywhere. */
+ * n_heads is a multiple of n_kv_heads, at most 16 query heads to a KV head; query head h uses KV head h /
+ * (n_heads / n_kv_heads).  head_size is 64 or 128.  Scores are q . k / sqrt(head_size), as everywhere. */
 
 /* Element types of activations. */
 enum { LPP_F32 = 0, LPP_F16 = 1 };
 
-/* Causal attention of whole prompts, packed one behind the other: rows d_offsets[s] .. d_offsets[s + 1] - 1 are sequence s,
- * and a row attends to the rows of its own sequence up to itself.  d_offsets: n_seqs + 1 ints that do not decrease, the
- * first 0 or more, the last n_tokens or less (values outside are cut to that range); sequences of no rows are
- * allowed.  NULL: one sequence of n_tokens rows (n_seqs is 1 then).  Rows of d_out that no sequence has are left as they
- * were.
- * q and out: [n_tokens][n_heads * head_size] of `type`; k and v: binary16 [n_tokens][n_kv_heads * head_size], what the
- * caches hold; the strides are the elements from one row to the next, kv_stride at most 2^24.  Rows start at multiples of
- * 16 bytes.  d_out must not overlap the inputs.  LPP_F32: queries and weights enter the products as binary16 head and
- * remainder, as in LPP_PREFILL_EXACT (a query beyond +-65504 gives NaN); LPP_F16: the weights are rounded to binary16 where V is weighted, sums are
- * fp32, the output is rounded once.  What K and V rows hold that a row does not attend to does not reach it, infinities
- * and NaN included; an infinity among the V values it does attend to gives an infinity or NaN.  The same inputs give the
- * same bits. */
+/* Causal attention of whole prompts, packed one behind the other: rows d_offsets[s] .. d_offsets[s + 1] - 1 are
+ * sequence s, and a row attends to the rows of its own sequence up to itself.  d_offsets: n_seqs + 1 ints that
+ * do not decrease, the first 0 or more, the last n_tokens or less (values outside are cut to that range);
+ * sequences of no rows are allowed.  NULL: one sequence of n_tokens rows (n_seqs is 1 then).  Rows of d_out
+ * that no sequence has are left as they were.
+ * q and out: [n_tokens][n_heads * head_size] of `type`; k and v: binary16 [n_tokens][n_kv_heads * head_size],
+ * what the caches hold; the strides are the elements from one row to the next, kv_stride at most 2^24.  Rows
+ * start at multiples of 16 bytes.  d_out must not overlap the inputs.  LPP_F32: queries and weights enter the
+ * products as binary16 head and remainder, as in LPP_PREFILL_EXACT (a query beyond +-65504 gives NaN); LPP_F16:
+ * the weights are rounded to binary16 where V is weighted, sums are fp32, the output is rounded once.  What K
+ * and V rows hold that a row does not attend to does not reach it, infinities and NaN included; an infinity
+ * among the V values it does attend to gives an infinity or NaN.  The same inputs give the same bits. */
 lpp_status lpp_prompt_attention(void *d_out, const void *d_q, const lpp_half *d_k, const lpp_half *d_v, int type,
                                 const int *d_offsets, int n_seqs, int n_tokens, int n_heads, int n_kv_heads,
                                 int head_size, int q_stride, int kv_stride, int out_stride);
 
-/* A cache of 4 bits.  A group is 32 values of a K or V row.  Its lowest value l is rounded to binary16, its scale c is
- * (highest - lowest) * (1 / 15) in fp32, rounded to binary16; a value's code is the integer nearest to (value - l) / c (ties to even,
- * 0 if c is 0), cut to 0 .. 15, and stands for l + code * c, rounded once to binary16.  A group with a value that is
- * not finite or beyond +-32768 stands for NaN throughout, so that an overflow shows.  5 bits a value in all.
- * One buffer of lpp_kv4_bytes() bytes, 16-byte aligned, in four parts: codes of K, codes of V, scales of K, scales of V, each
- * [n_layers][n_seqs][n_kv_heads][seq_len] and then head_size / 2 bytes of codes or head_size / 32 pairs of binary16 (scale,
- * lowest).  A 32-bit word of codes holds eight values: value 2 i at bit 4 i, value 2 i + 1 at bit 16 + 4 i. */
+/* A cache of 4 bits.  A group is 32 values of a K or V row.  Its lowest value l is rounded to binary16, its
+ * scale c is (highest - lowest) * (1 / 15) in fp32, rounded to binary16; a value's code is the integer nearest
+ * to (value - l) / c (ties to even, 0 if c is 0), cut to 0 .. 15, and stands for l + code * c, rounded once to
+ * binary16.  A group with a value that is not finite or beyond +-32768 stands for NaN throughout, so that an
+ * overflow shows.  5 bits a value in all. One buffer of lpp_kv4_bytes() bytes, 16-byte aligned, in four parts:
+ * codes of K, codes of V, scales of K, scales of V, each [n_layers][n_seqs][n_kv_heads][seq_len] and then
+ * head_size / 2 bytes of codes or head_size / 32 pairs of binary16 (scale, lowest).  A 32-bit word of codes
+ * holds eight values: value 2 i at bit 4 i, value 2 i + 1 at bit 16 + 4 i. */
 typedef struct lpp_kv4_shape {
     int n_layers;
     int n_seqs;
@@ -497,40 +498,43 @@ typedef struct lpp_kv4_shape {
 } lpp_kv4_shape;
 lpp_status lpp_kv4_bytes(const lpp_kv4_shape *shape, size_t *bytes);
 
-/* Rows of K and V into one layer of the cache.  k and v: [n_tokens][n_kv_heads * head_size] of `type`, rows at multiples of 16
- * bytes, kv_stride elements apart.  Rows d_offsets[s] .. d_offsets[s + 1] - 1 are sequence s's, as above; NULL: n_tokens / n_seqs
- * rows each.  The j-th of them goes to position d_starts[s] + j (d_starts NULL: j); a row whose position is not within
- * 0 .. seq_len - 1 is dropped, so a start of -n for n rows skips a sequence. */
+/* Rows of K and V into one layer of the cache.  k and v: [n_tokens][n_kv_heads * head_size] of `type`, rows at
+ * multiples of 16 bytes, kv_stride elements apart.  Rows d_offsets[s] .. d_offsets[s + 1] - 1 are sequence s's,
+ * as above; NULL: n_tokens / n_seqs rows each.  The j-th of them goes to position d_starts[s] + j (d_starts
+ * NULL: j); a row whose position is not within 0 .. seq_len - 1 is dropped, so a start of -n for n rows skips a
+ * sequence. */
 lpp_status lpp_kv4_store(void *d_cache, const lpp_kv4_shape *shape, int layer, const void *d_k, const void *d_v, int type,
                          int kv_stride, const int *d_offsets, int n_tokens, const int *d_starts);
 
 /* The binary16 numbers that positions first .. first + count - 1 of every sequence stand for: k and v
- * [n_seqs][n_kv_heads][count][head_size], 16-byte aligned (for one sequence and all positions: a layer of the model's own caches). */
+ * [n_seqs][n_kv_heads][count][head_size], 16-byte aligned (for one sequence and all positions: a layer of the
+ * model's own caches). */
 lpp_status lpp_kv4_load(lpp_half *d_k, lpp_half *d_v, const void *d_cache, const lpp_kv4_shape *shape, int layer,
                         int first, int count);
 
-/* Attention of n_q new rows a sequence over one layer of the cache, which holds them already: row j attends to positions
- * 0 .. d_starts[s] + j, with the d_starts that the store was given (cut to the positions there are; a row that attends to
- * none gives zeros).  q and out: fp32 [n_seqs][n_q][n_heads * head_size], 16-byte aligned, not overlapping, a query beyond
- * +-65504 gives NaN.  n_q = 1 is a decode step.
- * d_mass (may be NULL): fp32 [n_layers][n_seqs][n_kv_heads][seq_len]; to every position is added the weight it got, summed
- * over the rows and the query heads of its KV head.  Set it to zero when a sequence begins.
- * d_workspace: lpp_kv4_attention_workspace() bytes, 16-byte aligned, apart from all else; it need not be set to anything,
- * and calls that may run at the same time need one each.  The bytes grow with seq_len, n_heads and n_q, not with n_layers: one workspace
- * serves all layers.  The same inputs give the same bits. */
+/* Attention of n_q new rows a sequence over one layer of the cache, which holds them already: row j attends to
+ * positions 0 .. d_starts[s] + j, with the d_starts that the store was given (cut to the positions there are; a
+ * row that attends to none gives zeros).  q and out: fp32 [n_seqs][n_q][n_heads * head_size], 16-byte aligned,
+ * not overlapping, a query beyond +-65504 gives NaN.  n_q = 1 is a decode step.
+ * d_mass (may be NULL): fp32 [n_layers][n_seqs][n_kv_heads][seq_len]; to every position is added the weight it
+ * got, summed over the rows and the query heads of its KV head.  Set it to zero when a sequence begins.
+ * d_workspace: lpp_kv4_attention_workspace() bytes, 16-byte aligned, apart from all else; it need not be set to
+ * anything, and calls that may run at the same time need one each.  The bytes grow with seq_len, n_heads and
+ * n_q, not with n_layers: one workspace serves all layers.  The same inputs give the same bits. */
 lpp_status lpp_kv4_attention_workspace(const lpp_kv4_shape *shape, int n_heads, int n_q, size_t *bytes);
 lpp_status lpp_kv4_attention(float *d_out, const float *d_q, const void *d_cache, const lpp_kv4_shape *shape, int layer,
                              int n_heads, int n_q, const int *d_starts, float *d_mass, void *d_workspace,
                              size_t workspace_bytes);
 
-/* One layer of a cache reduced to `keep` positions of every (sequence, KV head), into a layer of another cache, whose
- * buffer must not overlap the first's: with n the sequence's d_lengths (cut to 0 .. seq_len), all positions if n <= keep;
- * else the last `recent` and, of the others, the keep - recent whose d_mass is largest (equal ones: the lower position;
- * NaN counts as largest), in the order they had.  Their rows go to positions 0 .. of d_dst, their mass to d_dst_mass,
- * whose further positions up to dst->seq_len are set to zero; rows behind the kept ones stay as they were.
- * d_dst_lengths[s] = min(n, keep).  d_kept: [n_seqs][n_kv_heads][keep], the position each kept row had, -1 behind them.
- * The shapes differ in n_layers and seq_len at most; 0 <= recent <= keep <= dst->seq_len.  d_dst_lengths must not be
- * d_lengths, nor d_dst_mass d_mass: the lengths are the same for every layer, and the next layer's call reads them again. */
+/* One layer of a cache reduced to `keep` positions of every (sequence, KV head), into a layer of another cache,
+ * whose buffer must not overlap the first's: with n the sequence's d_lengths (cut to 0 .. seq_len), all
+ * positions if n <= keep; else the last `recent` and, of the others, the keep - recent whose d_mass is largest
+ * (equal ones: the lower position; NaN counts as largest), in the order they had.  Their rows go to positions 0
+ * .. of d_dst, their mass to d_dst_mass, whose further positions up to dst->seq_len are set to zero; rows
+ * behind the kept ones stay as they were. d_dst_lengths[s] = min(n, keep).  d_kept: [n_seqs][n_kv_heads][keep],
+ * the position each kept row had, -1 behind them. The shapes differ in n_layers and seq_len at most; 0 <=
+ * recent <= keep <= dst->seq_len.  d_dst_lengths must not be d_lengths, nor d_dst_mass d_mass: the lengths are
+ * the same for every layer, and the next layer's call reads them again. */
 lpp_status lpp_kv4_evict(void *d_dst, const lpp_kv4_shape *dst, int dst_layer, float *d_dst_mass, int *d_dst_lengths,
                          int *d_kept, const void *d_src, const lpp_kv4_shape *src, int src_layer, const float *d_mass,
                          const int *d_lengths, int keep, int recent);

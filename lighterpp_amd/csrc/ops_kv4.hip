@@ -23,11 +23,11 @@ __device__ __forceinline__ int quad_or(int v) {
     return v | dpp_move_i<kDppXor2>(v);
 }
 
-// A word of the codes of eight values: the integers nearest to (x - low) / scale, in 0 .. 15.  In fp32, as fifteen times a number that is cut to
-// 0 .. 1 as it is formed, the quotient is off by less than 15 * 4 * 2^-24 and by 2^-22 of low / scale; a word with a quotient nearer than that to a
-// border (within 1e-5 and 2^-21) is formed again by the sign of x - low - border * scale.  (Of fp32 values that is one word in 6000; binary16 values lie
-// on a border itself often, about one word in 300.)  Adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the
-// lowest bits: the codes are added up with what is above them, which is taken off at the end.
+// A word of the codes of eight values: the integers nearest to (x - low) / scale, in 0 .. 15.  In fp32, as fifteen times a number that is cut to 0 ..
+// 1 as it is formed, the quotient is off by less than 15 * 4 * 2^-24 and by 2^-22 of low / scale; a word with a quotient nearer than that to a border
+// (within 1e-5 and 2^-21) is formed again by the sign of x - low - border * scale.  (Of fp32 values that is one word in 6000; binary16 values lie on
+// a border itself often, about one word in 300.)  Adding 2^23 rounds to the nearest integer, ties to even, and leaves it in the lowest bits: the
+// codes are added up with what is above them, which is taken off at the end.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], float low, float scale) {
     const float inverse = scale > 0.0f ? __builtin_amdgcn_rcpf(scale) : 0.0f;
     const float slope = inverse * (1.0f / 15.0f), shift = -low * slope;
@@ -203,11 +203,11 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
     return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
 }
 
-// One workgroup per sequence and KV head: the keep - recent positions of largest weight among the first n - recent, then the list in order.
-// The smallest weight kept is found by its bits, 11, 11 and 10 at a time from the top: counts of every value of those bits among the weights
-// that agree with what is known, added up from above.  A thread holds kHeld weights in registers (kOnce: all it has; else
-// stretches of them, read again in every pass).  A sequence and KV head of 2048 positions: 7.7 us, 128 of up to 8100 11 us, the time of its passes one
-// after the other; fewer threads are no faster.
+// One workgroup per sequence and KV head: the keep - recent positions of largest weight among the first n - recent, then the list in order. The
+// smallest weight kept is found by its bits, 11, 11 and 10 at a time from the top: counts of every value of those bits among the weights that agree
+// with what is known, added up from above.  A thread holds kHeld weights in registers (kOnce: all it has; else stretches of them, read again in every
+// pass).  A sequence and KV head of 2048 positions: 7.7 us, 128 of up to 8100 11 us, the time of its passes one after the other; fewer threads are no
+// faster.
 constexpr int kBins = 2048;
 template <int kHeld, bool kOnce>
 __global__ __launch_bounds__(kSelectThreads) void select_kernel(int* __restrict__ kept, int* __restrict__ dst_lengths, const float* __restrict__ mass,

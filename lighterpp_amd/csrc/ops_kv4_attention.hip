@@ -1,20 +1,18 @@
 // ops_kv4_attention.hip -- lpp_kv4_attention, lpp_kv4_attention_workspace:
-// attention of a few new rows over the cache of 4 bits, and the weight each
-// position got.
+// attention of a few new rows over the cache of 4 bits, and the weight each position got.
 //
 // The sums are those of a softmax in one walk: w(t, p) = 2^(scale q[t] . k[p] - top(t)), with `top` a score of the row so far, moved (and sum and
-// output rescaled) when a score passes it by more than kSlack.  The positions of a sequence are cut into shares, which leave (top, sum, output)
-// each; a second kernel weighs those by 2^(top - largest top) and adds them up in their order.  The weight that a position got needs the
-// row's final maximum and sum, so it is the second kernel's too.
+// output rescaled) when a score passes it by more than kSlack.  The positions of a sequence are cut into shares, which leave (top, sum, output) each;
+// a second kernel weighs those by 2^(top - largest top) and adds them up in their order.  The weight that a position got needs the row's final
+// maximum and sum, so it is the second kernel's too.
 //
-// What there is to read is 5 bits a value, K and V once for all the query heads of a KV head: 13 instructions make eight binary16 values of a
-// word of codes (dev::Kv4Reader), and the matrix cores take 16 rows x 16 positions at a time, the few rows there are beside unused ones, for which
-// nothing else would have to be formed.  Queries and weights enter as binary16 head and remainder.  V goes through LDS, for transposing
-// reads.
+// What there is to read is 5 bits a value, K and V once for all the query heads of a KV head: 13 instructions make eight binary16 values of a word of
+// codes (dev::Kv4Reader), and the matrix cores take 16 rows x 16 positions at a time, the few rows there are beside unused ones, for which nothing
+// else would have to be formed.  Queries and weights enter as binary16 head and remainder.  V goes through LDS, for transposing reads.
 //
 // What bounds it: 32 sequences of up to 8000 positions, 32 heads of 128 on 8: 60 us with the scores kept for the account (3.4 TB/s of the 160 bytes a
-// position and KV head; reading alone takes 47), and 9 for it and the merge; the rest is instructions for the codes.  One sequence of 16001, heads of 64: 7.6 + 3 us, one of 500:
-// 6.5 us: the time of requests one after the other, a start and a merge.
+// position and KV head; reading alone takes 47), and 9 for it and the merge; the rest is instructions for the codes.  One sequence of 16001, heads of
+// 64: 7.6 + 3 us, one of 500: 6.5 us: the time of requests one after the other, a start and a merge.
 #include "kv4.hpp"
 
 namespace lpp {
@@ -54,7 +52,10 @@ struct AttendJob {
     __device__ __forceinline__ int shares_of(int positions) const {
         float all = n_seqs > 4 * kWave ? static_cast<float>(positions) * n_seqs : 0.0f;
         if (n_seqs <= 4 * kWave)
-            for (int s0 = 0; s0 < n_seqs; s0 += kWave) all += wave_sum(s0 + lane_id() < n_seqs ? static_cast<float>(end_of(start_of(s0 + lane_id()), n_q - 1)) : 0.0f);
+            for (int s0 = 0; s0 < n_seqs; s0 += kWave) {
+                const int s = s0 + lane_id();
+                all += wave_sum(s < n_seqs ? static_cast<float>(end_of(start_of(s), n_q - 1)) : 0.0f);
+            }
         const int each = max(least, static_cast<int>(fminf(all * per_workgroup, 1e9f)));
         return max(min((positions + each - 1) / each, splits), 1);
     }
@@ -322,7 +323,8 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
         float step_sum = 0.0f;  // (of its own, so that the running sum is rounded once a step)
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-            const float p_0 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], scale, -top)), p_1 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][(e & 3) + 1], scale, -top));
+            const float p_0 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], scale, -top));
+            const float p_1 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][(e & 3) + 1], scale, -top));
             step_sum += p_0 + p_1;
             // (hidden from the compiler, which would otherwise round every value a second time to subtract it)
             uint32_t packed = __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(p_0), static_cast<half_t>(p_1)});
@@ -656,10 +658,10 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(AttendJob job, i
 
 int tiles_of(int n_q, int shared) { return (n_q + kRows / shared - 1) / (kRows / shared); }
 
-// Shares a sequence's positions are cut into at most, the least positions of one, the wavefronts to one, and how many of them run at once.
-// Few heads: 8 wavefronts to a share, for half the steps of each (one sequence of 8 KV heads of 64, us at 500 / 1000 / 8000 positions: 6.4 / 9.3 / 9.4,
-// 6.8 / 9.7 / 9.8 with 4 and 6.7 / 9.6 / 9.8 with 16; of 128: 8.2 / 10.9 / 11.4, 9.4 / 12.2 / 12.6 with 4).  512 positions at least: 256
-// or 1024 give one sequence of 16001 10.1 or 9.7 us for 8.0, and more or fewer shares to merge.
+// Shares a sequence's positions are cut into at most, the least positions of one, the wavefronts to one, and how many of them run at once. Few heads:
+// 8 wavefronts to a share, for half the steps of each (one sequence of 8 KV heads of 64, us at 500 / 1000 / 8000 positions: 6.4 / 9.3 / 9.4, 6.8 /
+// 9.7 / 9.8 with 4 and 6.7 / 9.6 / 9.8 with 16; of 128: 8.2 / 10.9 / 11.4, 9.4 / 12.2 / 12.6 with 4).  512 positions at least: 256 or 1024 give one
+// sequence of 16001 10.1 or 9.7 us for 8.0, and more or fewer shares to merge.
 struct Split {
     int splits, least, waves, workgroups;
 };
@@ -677,10 +679,10 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
 }
 
 // What the workspace holds.  Scores kept for the account are 4 bytes for every position and row; made from K again they cost its bytes and the
-// products (32 sequences of up to 8000 positions, 4 rows to a KV head of 128: 49 us more than without an account, and 10 so).  Not of several tiles, whose
-// scores are many times a layer (16 rows of 32 heads, 4 sequences of up to 3000 positions, heads of 64: 27.5 us for 25.5), and only where
-// the workspace gets no larger than partial results of kMaxSplits shares would make it: up to 14000 positions with four rows to a KV head of 64,
-// 2000 with sixteen.
+// products (32 sequences of up to 8000 positions, 4 rows to a KV head of 128: 49 us more than without an account, and 10 so).  Not of several tiles,
+// whose scores are many times a layer (16 rows of 32 heads, 4 sequences of up to 3000 positions, heads of 64: 27.5 us for 25.5), and only where the
+// workspace gets no larger than partial results of kMaxSplits shares would make it: up to 14000 positions with four rows to a KV head of 64, 2000
+// with sixteen.
 struct Workspace {
     size_t stats, partials, scores;  // floats
     int rows, steps;
@@ -742,7 +744,8 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     LPP_TRY(kv4_check_cache("lpp_kv4_attention", d_cache, shape, layer));
     LPP_TRY(check("lpp_kv4_attention", shape, n_heads, n_q));
     LPP_REQUIRE(d_out && d_q && d_starts && d_workspace, "lpp_kv4_attention: null pointer");
-    LPP_REQUIRE(reinterpret_cast<uintptr_t>(d_out) % 16 == 0 && reinterpret_cast<uintptr_t>(d_q) % 16 == 0 && reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0,
+    const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    LPP_REQUIRE(aligned(d_out) && aligned(d_q) && aligned(d_workspace),
                 "lpp_kv4_attention: d_out, d_q and d_workspace must start at multiples of 16 bytes");
     size_t need = 0;
     LPP_TRY(lpp_kv4_attention_workspace(shape, n_heads, n_q, &need));
@@ -772,9 +775,9 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     const Split split = split_of(*shape, job.tiles);
     job.splits = split.splits;
     job.least = split.least;
-    // Of many heads a quarter more shares than run at once: they are of unequal length, and the last to begin are not the last to end.  us for 1 / 1.25 /
-    // 1.5 / 2 times as many, heads of 128, ragged: 32 sequences of up to 8000 positions 62 / 59 / 56 / 58, 64 of 4000 60 / 58 / 58 / 59; 32 of 4000 alike 43 / 41.  Of few
-    // heads no more than run at once: 4 sequences of 8000 alike 17 / 23.
+    // Of many heads a quarter more shares than run at once: they are of unequal length, and the last to begin are not the last to end.  us for 1 /
+    // 1.25 / 1.5 / 2 times as many, heads of 128, ragged: 32 sequences of up to 8000 positions 62 / 59 / 56 / 58, 64 of 4000 60 / 58 / 58 / 59; 32 of
+    // 4000 alike 43 / 41.  Of few heads no more than run at once: 4 sequences of 8000 alike 17 / 23.
     job.per_workgroup = static_cast<float>(shape->n_kv_heads) * job.tiles / (split.waves == 4 ? 1.25f * split.workgroups : split.workgroups);
     job.per_shared = (65536u + job.shared - 1) / job.shared;
     const Workspace parts(*shape, n_q, job.shared, job.tiles, job.splits);
@@ -784,7 +787,8 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     job.partials = static_cast<float*>(d_workspace) + parts.stats;
     job.scores = d_mass != nullptr && parts.scores > 0 ? job.partials + parts.partials : nullptr;
     const long long groups = static_cast<long long>(job.heads) * job.tiles * job.splits;
-    LPP_REQUIRE(groups * dev::kWave * split.waves < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads and %d rows are too many for a launch", job.heads, n_q);
+    LPP_REQUIRE(groups * dev::kWave * split.waves < (1ll << 32),
+                "lpp_kv4_attention: %u sequences times KV heads and %d rows are too many for a launch", job.heads, n_q);
     const dim3 grid(static_cast<unsigned>(groups));
     if (shape->head_size == 64)
         LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
@@ -801,8 +805,8 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     }
     const int accounts = d_mass != nullptr ? (shape->seq_len + span - 1) / span : 0, blocks = merges + accounts;
     if (blocks > 0) {
-        LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32), "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch",
-                    job.heads, shape->seq_len);
+        LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32),
+                    "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch", job.heads, shape->seq_len);
         const auto kernel = shape->head_size == 64 ? (kept ? &finish_kernel<64, true> : &finish_kernel<64, false>)
                                                    : (kept ? &finish_kernel<128, true> : &finish_kernel<128, false>);
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, accounts, span);

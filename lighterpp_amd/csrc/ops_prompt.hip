@@ -5,18 +5,17 @@
 // log2(e) / sqrt(head_size).  One walk over the positions: `top` is a score of the row so far, moved (and sum and output rescaled) only when a score
 // passes it by more than kSlack; any value near the maximum would do, since it cancels.
 //
-// Both products run on the matrix cores, 32 positions x 32 query rows at a time: scores = K Q^T, whose result has a query row to a
-// lane and its positions in that lane's registers, as the second product, V^T W^T, wants its second operand; so weights never leave
-// registers, and maximum and sum of a row are two lanes' business.  The order in which the first product's rows come out is made good by the order in which
-// transposing reads take V rows from LDS.  fp32: queries and weights enter as binary16 head and remainder, twice the products.
+// Both products run on the matrix cores, 32 positions x 32 query rows at a time: scores = K Q^T, whose result has a query row to a lane and its
+// positions in that lane's registers, as the second product, V^T W^T, wants its second operand; so weights never leave registers, and maximum and sum
+// of a row are two lanes' business.  The order in which the first product's rows come out is made good by the order in which transposing reads take V
+// rows from LDS.  fp32: queries and weights enter as binary16 head and remainder, twice the products.
 //
-// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 548 to 585 us (machines hold different
-// clocks), 940 to 1000 TFLOP/s, where a matrix product of 8192^3 reaches 1186; the matrix cores are busy 49 % of
-// the cycles, vector ALUs 41 %, LDS 25 %, and fewer cycles cost clock.  Weights without exponentials, no maximum,
-// or no multiplication by the scale gain 0 to 10 %; two query tiles to a wavefront, for half the reads of LDS, are slower (half the
-// wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of 128 do not fit the registers).  Several pages (7 of up to 1500 rows, 32
-// heads of 64 on 8, fp32): 111 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us, the time of the requests one
-// after the other: offsets, rows, and the write.
+// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 548 to 585 us (machines hold different clocks), 940 to 1000 TFLOP/s,
+// where a matrix product of 8192^3 reaches 1186; the matrix cores are busy 49 % of the cycles, vector ALUs 41 %, LDS 25 %, and fewer cycles cost
+// clock.  Weights without exponentials, no maximum, or no multiplication by the scale gain 0 to 10 %; two query tiles to a wavefront, for half the
+// reads of LDS, are slower (half the wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of 128 do not fit the registers).  Several
+// pages (7 of up to 1500 rows, 32 heads of 64 on 8, fp32): 111 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us,
+// the time of the requests one after the other: offsets, rows, and the write.
 #include <type_traits>
 
 #include "kv4.hpp"
@@ -417,7 +416,11 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
         }
     };
     constexpr int kFours = kHs / 8;
-    auto four_of = [&](int four) { return floatx4{o[four >> 2][4 * (four & 3)], o[four >> 2][4 * (four & 3) + 1], o[four >> 2][4 * (four & 3) + 2], o[four >> 2][4 * (four & 3) + 3]}; };
+    auto four_of = [&](int four) {
+        const floatx16& of = o[four >> 2];
+        const int at = 4 * (four & 3);
+        return floatx4{of[at], of[at + 1], of[at + 2], of[at + 3]};
+    };
     if constexpr (kP == 1) {
         if (!valid) return;
         const float inv_sum = 1.0f / lsum;
@@ -487,12 +490,12 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
     return LPP_OK;
 }
 
-// Which shape: the fewer tiles of 32 rows there are for each compute unit, the more wavefronts share a walk.  us, one prompt, 1 x 4 / 2 x 2 /
-// 4 x 1, 32 heads of 64 on 8, fp32: 256 rows (one tile a compute unit) 6.4 / 7.9 / 10.3; 512 9.2 / 11.4 / 14.3; 700 16.0 / 14.3 / 16.6; 1024 21.1 /
-// 19.8 / 22.9; 1500 36.7 / 34.5 / 32.4; 2048 58 / 53 / 48; 6000 364 / 327 / 284.  32 heads of 128, binary16: 256 7.0 / 8.5 / 10.6; 400
-// 12.2 / 10.9 / 13.0; 1024 32 / 21 / 25; 1500 57 / 35.5 / 36.0; 2048 90 / 53 / 51; 6000 567 / 357 / 306.  Steps of 4 x 1: 128 positions (fp32, heads of
-// 64; 64: 302 us at 6000 rows for 292), 64 (binary16, heads of 128; 32: 350 for 321; heads of 64, where three workgroups fit on a compute unit so: 7 prompts of
-// up to 1500 rows 45 us, 49 with 128) or 32 (fp32, heads of 128, where 64 spill: the same prompts 122 us for 131).  (8 x 1: 326 and 331; the products of
+// Which shape: the fewer tiles of 32 rows there are for each compute unit, the more wavefronts share a walk.  us, one prompt, 1 x 4 / 2 x 2 / 4 x 1,
+// 32 heads of 64 on 8, fp32: 256 rows (one tile a compute unit) 6.4 / 7.9 / 10.3; 512 9.2 / 11.4 / 14.3; 700 16.0 / 14.3 / 16.6; 1024 21.1 / 19.8 /
+// 22.9; 1500 36.7 / 34.5 / 32.4; 2048 58 / 53 / 48; 6000 364 / 327 / 284.  32 heads of 128, binary16: 256 7.0 / 8.5 / 10.6; 400 12.2 / 10.9 / 13.0;
+// 1024 32 / 21 / 25; 1500 57 / 35.5 / 36.0; 2048 90 / 53 / 51; 6000 567 / 357 / 306.  Steps of 4 x 1: 128 positions (fp32, heads of 64; 64: 302 us at
+// 6000 rows for 292), 64 (binary16, heads of 128; 32: 350 for 321; heads of 64, where three workgroups fit on a compute unit so: 7 prompts of up to
+// 1500 rows 45 us, 49 with 128) or 32 (fp32, heads of 128, where 64 spill: the same prompts 122 us for 131).  (8 x 1: 326 and 331; the products of
 // the next step formed between this one's weights, this step's products and weights in turn, a third stage, or other priorities for the products: no
 // faster.)
 template <typename T, int kHs>
