@@ -70,6 +70,11 @@ inline lpp_status tell_lds(const void* kernel, int bytes, bool (&told)[64]) {
 
 namespace dev {
 
+// A softmax in one walk takes its weights as 2^(score - reference).  The reference lies kLift below a score of the row and moves when a score passes that
+// one by more than kSlack: the largest weight is between 2^8 and 2^15, near binary16's largest, so that small ones keep bits in its subnormals (2^-33
+// of the largest weight, head and remainder).
+constexpr float kLift = 9.0f, kSlack = 6.0f;
+
 // The eight binary16 numbers that a word of codes stands for.  A code in the last bits of a half whose exponent is that of 1024 is
 // 1024 + code, four bits further up and with the exponent of 64 it is 64 + code: a pair costs one and-or, one (exact) subtraction and one
 // fused multiply-add, the one rounding, and a word one shift.

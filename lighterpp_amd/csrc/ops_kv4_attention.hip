@@ -26,7 +26,6 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 constexpr int kRows = 16;       // of a tile: (16 / shared) new rows x the query heads of a KV head
 constexpr int kStep = 32;       // positions a wavefront takes at a time
 constexpr int kMaxSplits = 64;  // shares that a sequence's positions are cut into
-constexpr float kSlack = 6.0f;  // weights stay below 2^6: far from fp32's limits and binary16's largest
 
 struct AttendJob {
     float* out;
@@ -249,7 +248,7 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     for (int dt = 0; dt < kDTiles; ++dt) o[dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
     float top = 0.0f, lsum = 0.0f;  // (the sum over this lane's own positions)
-    bool seen = false;              // the row has attended to something: top is a score
+    bool seen = false;              // the row has attended to something: top is a score less kLift
     float minus_one = -1.0f;
     asm("" : "+v"(minus_one));
 
@@ -309,9 +308,9 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
 #pragma unroll
             for (int e = 0; e < 4; ++e) step_top = fmaxf(step_top, st[t][e]);
         step_top = __builtin_ceilf(rows_max(step_top) * scale);
-        const bool moves = step_top > (seen ? top + kSlack : -INFINITY);
+        const bool moves = step_top > (seen ? top + (kLift + kSlack) : -INFINITY);
         if (__builtin_amdgcn_ballot_w64(moves) != 0ull) {  // (uniform)
-            const float to = moves ? step_top : top;
+            const float to = moves ? step_top - kLift : top;
             const float corr = __builtin_amdgcn_exp2f(seen ? top - to : 0.0f);  // (nothing to rescale before a row's first step)
             top = to;
             lsum *= corr;

@@ -220,10 +220,9 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
     for (int dt = 0; dt < kDTiles; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
-    constexpr float kSlack = 6.0f;  // weights stay below 2^6: their sums are far from fp32's limits, and in binary16 from its largest
     const float scale = 1.44269504088896341f / sqrtf(static_cast<float>(kHs));
     float top = 0.0f, lsum = 0.0f;  // (the sum over this lane's own positions)
-    bool seen = false;              // the row has attended to something: top is a score
+    bool seen = false;              // the row has attended to something: top is a score less kLift
     float minus_one = -1.0f;
     asm("" : "+v"(minus_one));
 
@@ -292,9 +291,9 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
             for (int e = 0; e < 16; ++e) step_top = fmaxf(step_top, st[t][e]);
         step_top = halves_max(step_top) * scale;
         if constexpr (kLo) step_top = __builtin_ceilf(step_top);
-        const bool moves = step_top > (seen ? top + kSlack : -INFINITY);
+        const bool moves = step_top > (seen ? top + (kLift + kSlack) : -INFINITY);
         if (__builtin_amdgcn_ballot_w64(moves) != 0ull) {  // (uniform)
-            const float to = moves ? step_top : top;
+            const float to = moves ? step_top - kLift : top;
             const float corr = __builtin_amdgcn_exp2f(seen ? top - to : 0.0f);  // (nothing to rescale before a row's first step)
             top = to;
             lsum *= corr;

@@ -323,6 +323,21 @@ def test_large_scores(lib, hs):
     check_attention(got, got_mass, cache, 0, q, [room - 1, room - 1], mass)
 
 
+@pytest.mark.parametrize("hs", [64, 128])
+def test_small_weights_alone(lib, hs):
+    """Nearly all of the weight lies where V is zero: what is left is the share of weights of 2^-12 to 2^-18, with their own accuracy."""
+    rng = np.random.default_rng(hs)
+    room, heads, scale = 40, 4, 8 / np.sqrt(hs)
+    cache = random_cache(rng, 1, 1, heads, room, hs)
+    for p in range(room):
+        k = np.full((heads, hs), 0.75 if p == 0 else -0.6, F) - (0 if p == 0 else rng.random((heads, 1)).astype(F) * F(0.15))
+        cache.put(0, 0, 0, p, (k * scale).astype(F))
+        cache.put(1, 0, 0, p, np.zeros((heads, hs), F) if p == 0 else rng.standard_normal((heads, hs)).astype(F))
+    q = np.full((1, 3, heads, hs), scale, F) * (1 + rng.random((1, 3, heads, 1)).astype(F) * F(0.05))
+    got, _ = attend(lib, DB.from_numpy(cache.buffer), cache, 0, q, [room - 3])
+    check_attention(got, None, cache, 0, q, [room - 3], None)
+
+
 @pytest.mark.parametrize("heads,kv,hs", [(4, 4, 64), (8, 1, 64), (6, 2, 128)])
 @pytest.mark.parametrize("n_q", [1, 5])
 @pytest.mark.parametrize("where", [0, 1])

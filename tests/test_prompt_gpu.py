@@ -172,6 +172,21 @@ def test_nothing_comes_from_positions_a_row_does_not_attend_to(lib, where, bad, 
         assert np.isnan(got[seen]).all()
 
 
+@pytest.mark.parametrize("hs", [64, 128])
+def test_small_weights_alone(lib, hs):
+    """Nearly all of the weight lies where V is zero: what is left is the share of weights of 2^-12 to 2^-18, with their own accuracy."""
+    rng = np.random.default_rng(hs)
+    rows, heads = 40, 4
+    q = np.full((rows, heads, hs), 8 / np.sqrt(hs), F) * (1 + rng.random((rows, heads, 1)).astype(F) * F(0.05))
+    k = np.full((rows, heads, hs), -0.6, H) - rng.random((rows, heads, 1)).astype(H) * H(0.15)
+    k[0] = H(0.75) * H(8 / np.sqrt(hs))
+    k[1:] = k[1:] * H(8 / np.sqrt(hs))
+    v = rng.standard_normal((rows, heads, hs)).astype(H)
+    v[0] = 0
+    with np.errstate(invalid="ignore"):  # (row 0 is zero, and so is its tolerance)
+        against(run(lib, q, k, v, [0, rows]), q, k, v, [(0, rows)])
+
+
 def test_same_bits_twice(lib):
     q, k, v = inputs(11, 700, 8, 2, 64, F)
     a, b = run(lib, q, k, v, [0, 100, 700]), run(lib, q, k, v, [0, 100, 700])
