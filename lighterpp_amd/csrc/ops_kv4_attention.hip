@@ -1,8 +1,8 @@
 // ops_kv4_attention.hip -- lpp_kv4_attention, lpp_kv4_attention_workspace:
 // attention of a few new rows over the cache of 4 bits, and the weight each position got.
 //
-// The sums are those of a softmax in one walk: w(t, p) = 2^(scale q[t] . k[p] - top(t)), with `top` a score of the row so far, moved (and sum and
-// output rescaled) when a score passes it by more than kSlack.  The positions of a sequence are cut into shares, which leave (top, sum, output) each;
+// The sums are those of a softmax in one walk: w(t, p) = 2^(scale q[t] . k[p] - top(t)), with `top` kLift below a score of the row so far, moved
+// (and sum and output rescaled) when a score passes that one by more than kSlack.  The positions of a sequence are cut into shares, which leave (top, sum, output) each;
 // a second kernel weighs those by 2^(top - largest top) and adds them up in their order.  The weight that a position got needs the row's final
 // maximum and sum, so it is the second kernel's too.
 //

@@ -2,8 +2,8 @@
 // packed one behind the other.
 //
 // out[t] = sum_p w(t, p) v[p] / sum_p w(t, p) with w(t, p) = 2^(scale q[t] . k[p] - top(t)), over the positions p <= t of t's sequence, scale =
-// log2(e) / sqrt(head_size).  One walk over the positions: `top` is a score of the row so far, moved (and sum and output rescaled) only when a score
-// passes it by more than kSlack; any value near the maximum would do, since it cancels.
+// log2(e) / sqrt(head_size).  One walk over the positions: `top` lies kLift below a score of the row so far, and moves (sum and output are rescaled) only when a
+// score passes that one by more than kSlack; any value near the maximum would do, since it cancels.
 //
 // Both products run on the matrix cores, 32 positions x 32 query rows at a time: scores = K Q^T, whose result has a query row to a lane and its
 // positions in that lane's registers, as the second product, V^T W^T, wants its second operand; so weights never leave registers, and maximum and sum
