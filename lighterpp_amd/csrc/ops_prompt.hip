@@ -80,7 +80,8 @@ __device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_rea
 
 // The workgroup's tile: which of its sequence's tiles it is, and the sequence's rows (returned; 0: it has none).  Up to 64 sequences: in the order of
 // their walks' lengths, longest first, whatever the sequence.  More: sequence s's tiles, the last one first, from number
-// offsets[s] / tokens + s on, which leaves room for those of the sequences before.
+// offsets[s] / tokens + s on, which leaves room for those of the sequences before (s counts those without rows too, so the numbers run to n_tokens /
+// tokens + n_seqs).
 __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& tile, int& first_row) {
     if (job.offsets == nullptr) {
         first_row = 0;
@@ -479,11 +480,13 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
         static bool sized[64] = {};
         LPP_TRY(tell_lds(reinterpret_cast<const void*>(kernel), kLds, sized));
     }
-    // (as many tiles as sequences of any lengths can have)
+    // (as many tile numbers as find_tile gives to sequences of any lengths: one more than whole tiles for each sequence, and up to kWave of them only
+    // for those that have rows)
     const int tokens = kR * (32 / job.shared);
-    const long long tiles = job.n_tokens / tokens + (n_seqs < job.n_tokens ? n_seqs : job.n_tokens);
+    const long long tiles = job.n_tokens / tokens + (n_seqs <= dev::kWave && n_seqs > job.n_tokens ? job.n_tokens : n_seqs);
     const long long blocks = tiles * job.n_kv_heads;
-    LPP_REQUIRE(blocks * 64 * kR * kP < (1ll << 32), "lpp_prompt_attention: %d rows of %d KV heads are too many for a launch", job.n_tokens, job.n_kv_heads);
+    LPP_REQUIRE(blocks * 64 * kR * kP < (1ll << 32), "lpp_prompt_attention: %d rows of %d sequences and %d KV heads are too many for a launch", job.n_tokens,
+                n_seqs, job.n_kv_heads);
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(64 * kR * kP), kLds, stream(), job);
     LPP_CHECK_LAUNCH("prompt_kernel");
     return LPP_OK;

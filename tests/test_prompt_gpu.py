@@ -248,3 +248,21 @@ def test_captured_in_a_graph(lib, heads, kv, hs, typ):
     finally:
         capi.check(lib.lpp_set_stream(None))
         hip("hipStreamDestroy", side)
+
+
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("heads,kv,hs", [(8, 2, 64), (3, 3, 128), (16, 1, 64)])
+@pytest.mark.parametrize("lengths", [
+    {65: {64: 1}}, {128: {99: 30, 120: 20}}, {128: {s: 1 for s in range(0, 128, 3)}}, {100: {s: 1 for s in range(90, 100)}}, {71: {70: 50}},
+    {5000: {0: 3, 2500: 300, 4998: 1, 4999: 40}}, {300: {0: 40}}],
+    ids=["one_row_last", "two_of_128", "every_third", "ten_last", "one_prompt_last", "four_of_5000", "one_first"])
+def test_fewer_rows_than_sequences(lib, lengths, heads, kv, hs, typ):
+    """A table of slots, most of them without a prompt: the rows of every sequence that has some."""
+    (seqs, there), = lengths.items()
+    lengths = np.zeros(seqs, int)
+    for s, n in there.items():
+        lengths[s] = n
+    assert lengths.sum() < seqs
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = inputs(seqs + heads, int(offsets[-1]), heads, kv, hs, typ)
+    against(run(lib, q, k, v, offsets), q, k, v, list(zip(offsets[:-1], offsets[1:])))
