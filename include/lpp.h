@@ -472,11 +472,11 @@ enum { LPP_F32 = 0, LPP_F16 = 1 };
  * that no sequence has are left as they were.
  * q and out: [n_tokens][n_heads * head_size] of `type`; k and v: binary16 [n_tokens][n_kv_heads * head_size],
  * what the caches hold; the strides are the elements from one row to the next, kv_stride at most 2^24.  Rows
- * start at multiples of 16 bytes.  d_out must not overlap the inputs.  LPP_F32: queries and weights enter the
- * products as binary16 head and remainder, as in LPP_PREFILL_EXACT (a query beyond +-65504 gives NaN); LPP_F16:
- * the weights are rounded to binary16 where V is weighted, sums are fp32, the output is rounded once.  What K
- * and V rows hold that a row does not attend to does not reach it, infinities and NaN included; an infinity
- * among the V values it does attend to gives an infinity or NaN.  The same inputs give the same bits. */
+ * start at multiples of 16 bytes.  d_out must not overlap the inputs.  Queries (LPP_F32: as binary16 head and
+ * remainder, and a query beyond +-65504 gives NaN) and weights (as head and remainder) enter the products as in
+ * LPP_PREFILL_EXACT, sums are fp32, and LPP_F16 rounds the output, once.  What K and V rows hold that a row does
+ * not attend to does not reach it, infinities and NaN included; an infinity among the V values it does attend to
+ * gives an infinity or NaN.  The same inputs give the same bits. */
 lpp_status lpp_prompt_attention(void *d_out, const void *d_q, const lpp_half *d_k, const lpp_half *d_v, int type,
                                 const int *d_offsets, int n_seqs, int n_tokens, int n_heads, int n_kv_heads,
                                 int head_size, int q_stride, int kv_stride, int out_stride);

@@ -8,14 +8,16 @@
 // Both products run on the matrix cores, 32 positions x 32 query rows at a time: scores = K Q^T, whose result has a query row to a lane and its
 // positions in that lane's registers, as the second product, V^T W^T, wants its second operand; so weights never leave registers, and maximum and sum
 // of a row are two lanes' business.  The order in which the first product's rows come out is made good by the order in which transposing reads take V
-// rows from LDS.  fp32: queries and weights enter as binary16 head and remainder, twice the products.
+// rows from LDS.  Weights enter as binary16 head and remainder, and so do fp32 queries: the second product is twice its size, with fp32 the first too.
+// (Weights rounded to binary16 would be enough for binary16 activations by their size, but the output's error would be 2.4e-4 to 2.7e-4 of its norm where
+// its own rounding makes 2.0e-4; with the remainders it is rounded once, and is within 2e-5 of fp32 arithmetic rounded.  They cost 4 % with prompts of
+// 250 rows, a fifth at 2000 and a third at 8191.)
 //
-// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 548 to 585 us (machines hold different clocks), 940 to 1000 TFLOP/s,
-// where a matrix product of 8192^3 reaches 1186; the matrix cores are busy 49 % of the cycles, vector ALUs 41 %, LDS 25 %, and fewer cycles cost
-// clock.  Weights without exponentials, no maximum, or no multiplication by the scale gain 0 to 10 %; two query tiles to a wavefront, for half the
-// reads of LDS, are slower (half the wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of 128 do not fit the registers).  Several
-// pages (7 of up to 1500 rows, 32 heads of 64 on 8, fp32): 111 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us,
-// the time of the requests one after the other: offsets, rows, and the write.
+// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 731 us, 1130 TFLOP/s of products, where a matrix product of 8192^3
+// reaches 1186: matrix cores at the clock that the power leaves.  Without exponentials, a maximum, or the multiplication by the scale fp32 gained 0 to 10 %;
+// two query tiles to a wavefront, for half the reads of LDS, are slower (half the wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of
+// 128 do not fit the registers).  Several pages (7 of up to 1500 rows, 32 heads of 64 on 8, fp32): 111 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us, the
+// time of the requests one after the other: offsets, rows, and the write.
 #include <type_traits>
 
 #include "kv4.hpp"
@@ -124,7 +126,7 @@ __device__ __forceinline__ int find_tile(const PromptJob& job, int tokens, int& 
 template <typename T, int kHs, int kR, int kP, int kStepRows>
 __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) void prompt_kernel(PromptJob job) {
     typedef Shape<kHs, kR, kP, kStepRows> S;
-    constexpr bool kLo = sizeof(T) == 4;  // heads and remainders
+    constexpr bool kLo = sizeof(T) == 4;  // queries have a remainder
     constexpr int kDTiles = kHs / 32, kKSteps = kHs / 16, kStep = S::kStep, kRowBytes = S::kRowBytes, kPieces = S::kPieces;
     constexpr int kTiles = kStep / 32;  // tiles of 32 positions in a step
     extern __shared__ __align__(1024) char lds[];
@@ -335,22 +337,17 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 const float s_0 = st[s2 >> 1][8 * (s2 & 1) + e], s_1 = st[s2 >> 1][8 * (s2 & 1) + e + 1];
-                float p_0 = __builtin_amdgcn_exp2f(fmaf(s_0, scale, -top)), p_1 = __builtin_amdgcn_exp2f(fmaf(s_1, scale, -top));
+                const float p_0 = __builtin_amdgcn_exp2f(fmaf(s_0, scale, -top)), p_1 = __builtin_amdgcn_exp2f(fmaf(s_1, scale, -top));
                 // (the packed pair and the factor -1 are hidden from the compiler, which would otherwise round every value a second time to
                 // subtract it)
                 uint32_t packed = __builtin_bit_cast(uint32_t, half2_t{static_cast<half_t>(p_0), static_cast<half_t>(p_1)});
-                if constexpr (kLo) asm("" : "+v"(packed));
+                asm("" : "+v"(packed));
                 const half2_t h = __builtin_bit_cast(half2_t, packed);
                 ph[e] = h[0];
                 ph[e + 1] = h[1];
-                if constexpr (kLo) {
-                    step_sum += p_0 + p_1;
-                    pl[e] = static_cast<half_t>(fmaf(static_cast<float>(h[0]), minus_one, p_0));
-                    pl[e + 1] = static_cast<half_t>(fmaf(static_cast<float>(h[1]), minus_one, p_1));
-                } else {
-                    // (the sum of the rounded weights, which are what V is weighted with, two to an instruction)
-                    step_sum = __builtin_amdgcn_fdot2(h, half2_t{static_cast<half_t>(1.0f), static_cast<half_t>(1.0f)}, step_sum, false);
-                }
+                step_sum += p_0 + p_1;
+                pl[e] = static_cast<half_t>(fmaf(static_cast<float>(h[0]), minus_one, p_0));
+                pl[e + 1] = static_cast<half_t>(fmaf(static_cast<float>(h[1]), minus_one, p_1));
             }
             if (kPartly && odd) {
                 // (uniform) A weight of zero would not keep it out.  One token after the other, with the rows behind it cleared; a lane's output is
@@ -364,7 +361,7 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
                         for (int e = 0; e < 8; ++e)
                             if ((e & 3) + 8 * (e >> 2) >= end) seen_v[e] = static_cast<half_t>(0.0f);
                         floatx16 with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, ph, o[dt], 0, 0, 0);
-                        if constexpr (kLo) with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
+                        with = __builtin_amdgcn_mfma_f32_32x32x16_f16(seen_v, pl, with, 0, 0, 0);
                         if (my_tok == t0 + token) o[dt] = with;
                     }
                 }
@@ -373,7 +370,7 @@ __global__ __launch_bounds__(64 * kR * kP, sizeof(T) == 2 && kHs == 64 ? 3 : 2) 
                 for (int dt = 0; dt < kDTiles; ++dt) {
                     const half8_t v = values_of(s2, dt);
                     o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph, o[dt], 0, 0, 0);
-                    if constexpr (kLo) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl, o[dt], 0, 0, 0);
                 }
             }
         }
@@ -494,12 +491,13 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
 
 // Which shape: the fewer tiles of 32 rows there are for each compute unit, the more wavefronts share a walk.  us, one prompt, 1 x 4 / 2 x 2 / 4 x 1,
 // 32 heads of 64 on 8, fp32: 256 rows (one tile a compute unit) 6.4 / 7.9 / 10.3; 512 9.2 / 11.4 / 14.3; 700 16.0 / 14.3 / 16.6; 1024 21.1 / 19.8 /
-// 22.9; 1500 36.7 / 34.5 / 32.4; 2048 58 / 53 / 48; 6000 364 / 327 / 284.  32 heads of 128, binary16: 256 7.0 / 8.5 / 10.6; 400 12.2 / 10.9 / 13.0;
-// 1024 32 / 21 / 25; 1500 57 / 35.5 / 36.0; 2048 90 / 53 / 51; 6000 567 / 357 / 306.  Steps of 4 x 1: 128 positions (fp32, heads of 64; 64: 302 us at
-// 6000 rows for 292), 64 (binary16, heads of 128; 32: 350 for 321; heads of 64, where three workgroups fit on a compute unit so: 7 prompts of up to
-// 1500 rows 45 us, 49 with 128) or 32 (fp32, heads of 128, where 64 spill: the same prompts 122 us for 131).  (8 x 1: 326 and 331; the products of
-// the next step formed between this one's weights, this step's products and weights in turn, a third stage, or other priorities for the products: no
-// faster.)
+// 22.9; 1500 36.7 / 34.5 / 32.4; 2048 58 / 53 / 48; 6000 364 / 327 / 284.  32 heads of 128, binary16: 256 7.5 / 8.9 / 11.6; 400 13.2 / 11.8 / 14.7;
+// 1024 35 / 23 / 28.5; 1500 61 / 41 / 42; 2048 100 / 64 / 63; 6000 640 / 447 / 401; of 64: 512 7.4 / 9.2 / 11.8; 700 12.6 / 11.1 / 14.7; 1500 28 / 25 /
+// 27; 2048 45.5 / 39.2 / 38.6.  Steps of 4 x 1: 128 positions (fp32, heads of 64; 64: 302 us at 6000 rows for 292), 64 (binary16, heads of 128; 32: 410
+// for 401; heads of 64, where three workgroups fit on a compute unit so: 7 prompts of up to 1500 rows 53.6 us, 60 with 128) or 32 (fp32, heads of 128,
+// where 64 spill: the same prompts 122 us for 131).  (Built when binary16 weights had no remainder, 321 us at 6000 rows, and no faster: 8 x 1, 326
+// and 331; the products of the next step formed between this one's weights, this step's products and weights in turn, a third stage, other
+// priorities for the products.)
 template <typename T, int kHs>
 lpp_status launch(const PromptJob& job, int n_seqs) {
     const long long tiles = (static_cast<long long>(job.n_tokens) * job.shared + 31) / 32 * job.n_kv_heads;  // of 32 rows

@@ -266,3 +266,21 @@ def test_fewer_rows_than_sequences(lib, lengths, heads, kv, hs, typ):
     offsets = np.concatenate([[0], np.cumsum(lengths)])
     q, k, v = inputs(seqs + heads, int(offsets[-1]), heads, kv, hs, typ)
     against(run(lib, q, k, v, offsets), q, k, v, list(zip(offsets[:-1], offsets[1:])))
+
+
+@pytest.mark.parametrize("heads,kv,hs,lengths", [(8, 2, 64, [1, 45, 130, 300]), (6, 2, 128, [257, 90]), (32, 8, 64, [700]), (16, 8, 128, [900])])
+def test_binary16_is_rounded_once(lib, heads, kv, hs, lengths):
+    """Binary16 queries and output: the error of fp32 ones, and the one rounding of the output (half a step: 2^-11 of the value, 2^-25 where it is
+    subnormal).  A weight's remainder is kept to 2^-33 of its row's largest."""
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = inputs(sum(lengths) + heads, int(offsets[-1]), heads, kv, hs, H, spread=0.25)
+    got = run(lib, q, k, v, offsets).astype(np.float64)
+    for a, b in zip(offsets[:-1], offsets[1:]):
+        rows = np.unique(np.linspace(0, b - a - 1, 40).astype(int))
+        args = q[a:b][rows], k[a:b].transpose(1, 0, 2), v[a:b].transpose(1, 0, 2), [int(j) + 1 for j in rows]
+        want, weights, tol = ko.attend_tolerance(*args)
+        for h in range(heads):
+            tol[:, h] += weights[:, h].max(-1, keepdims=True) * 2.0 ** -33 * np.abs(v[a:b, h * kv // heads].astype(np.float64)).sum(0)
+        tol += (np.abs(want) + tol) * 2.0 ** -11 + 2.0 ** -25
+        off = np.abs(got[a:b][rows] - want)
+        assert np.all(off <= tol), (a, b, float((off / tol).max()))
