@@ -519,8 +519,9 @@ lpp_status lpp_kv4_load(lpp_half *d_k, lpp_half *d_v, const void *d_cache, const
  * d_mass (may be NULL): fp32 [n_layers][n_seqs][n_kv_heads][seq_len]; to every position is added the weight it
  * got, summed over the rows and the query heads of its KV head.  Set it to zero when a sequence begins.
  * d_workspace: lpp_kv4_attention_workspace() bytes, 16-byte aligned, apart from all else; it need not be set to
- * anything, and calls that may run at the same time need one each.  The bytes grow with seq_len, n_heads and
- * n_q, not with n_layers: one workspace serves all layers.  The same inputs give the same bits. */
+ * anything, and calls that may run at the same time need one each.  Fewer sequences, positions, query heads or
+ * rows never need more, and n_layers is not in it: a workspace of the largest call serves the others, and all
+ * layers.  The same inputs give the same bits. */
 lpp_status lpp_kv4_attention_workspace(const lpp_kv4_shape *shape, int n_heads, int n_q, size_t *bytes);
 lpp_status lpp_kv4_attention(float *d_out, const float *d_q, const void *d_cache, const lpp_kv4_shape *shape, int layer,
                              int n_heads, int n_q, const int *d_starts, float *d_mass, void *d_workspace,

@@ -663,6 +663,7 @@ int tiles_of(int n_q, int shared) { return (n_q + kRows / shared - 1) / (kRows /
 // sequence of 16001 10.1 or 9.7 us for 8.0, and more or fewer shares to merge.
 struct Split {
     int splits, least, waves, workgroups;
+    size_t most, rounds;  // shares of a sequence by its positions; of all tiles
 };
 Split split_of(const lpp_kv4_shape& shape, int tiles) {
     const long long heads = static_cast<long long>(shape.n_seqs) * shape.n_kv_heads * tiles;
@@ -670,9 +671,12 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
     s.waves = heads * 4 > compute_units() ? 4 : 8;
     s.least = 512;
     s.workgroups = compute_units() * (shape.head_size == 64 ? 16 / s.waves : s.waves == 8 ? 1 : 3);  // (by registers, and LDS for the heads of 128)
+    const int most = (shape.seq_len + s.least - 1) / s.least;
+    s.splits = most < kMaxSplits ? most : kMaxSplits;
+    s.most = s.splits;
     // (no more workgroups than 16 rounds of them, most of which would find no share)
-    const long long rounds = 16ll * s.workgroups / heads, most = (shape.seq_len + s.least - 1) / s.least;
-    s.splits = static_cast<int>(most < kMaxSplits ? most : kMaxSplits);
+    s.rounds = 16ull * s.workgroups;
+    const long long rounds = 16ll * s.workgroups / heads;
     if (s.splits > rounds) s.splits = static_cast<int>(rounds > 1 ? rounds : 1);
     return s;
 }
@@ -680,21 +684,31 @@ Split split_of(const lpp_kv4_shape& shape, int tiles) {
 // What the workspace holds.  Scores kept for the account are 4 bytes for every position and row; made from K again they cost its bytes and the
 // products (32 sequences of up to 8000 positions, 4 rows to a KV head of 128: 49 us more than without an account, and 10 so).  Not of several tiles,
 // whose scores are many times a layer (16 rows of 32 heads, 4 sequences of up to 3000 positions, heads of 64: 27.5 us for 25.5), and only where the
-// workspace gets no larger than partial results of kMaxSplits shares would make it: up to 14000 positions with four rows to a KV head of 64, 2000
-// with sixteen.
+// workspace gets no larger than partial results of kMaxSplits shares would make it: up to about 14900 positions with four rows to a KV head of 64,
+// 3680 with sixteen.
+// `bytes` is no less than that of any call of fewer sequences, positions, heads or rows, whose layout may take more than this one's (scores that this one
+// does not keep; shares, whose number is rounded down to what runs at once): one workspace serves them all.
 struct Workspace {
     size_t stats, partials, scores;  // floats
     int rows, steps;
-    size_t bytes() const { return (stats + partials + scores) * sizeof(float); }
-    Workspace(const lpp_kv4_shape& shape, int n_q, int shared, int tiles, int splits) {
-        const size_t all_tiles = static_cast<size_t>(shape.n_seqs) * shape.n_kv_heads * tiles;
+    size_t bytes;
+    Workspace(const lpp_kv4_shape& shape, int n_q, int shared, int tiles, const Split& split) {
+        const size_t heads = static_cast<size_t>(shape.n_seqs) * shape.n_kv_heads, all_tiles = heads * tiles;
         rows = (n_q < kRows / shared ? n_q : kRows / shared) * shared;
         steps = (shape.seq_len + kStep - 1) / kStep;
-        const size_t slots = static_cast<size_t>(splits) * rows, kept = static_cast<size_t>(rows) * steps * kStep;
-        const size_t sums = (slots * 2 + 3) / 4 * 4, outputs = slots * shape.head_size;
-        stats = all_tiles * sums;
-        partials = all_tiles * outputs;
-        scores = tiles == 1 && kept + sums + outputs <= static_cast<size_t>(kMaxSplits) * kRows * (shape.head_size + 2) ? all_tiles * kept : 0;
+        const size_t limit = heads * kMaxSplits * kRows * (shape.head_size + 2), of_scores = heads * steps * kStep;
+        const auto sums = [](size_t slots) { return (slots * 2 + 3) / 4 * 4; };
+        const size_t slots = all_tiles * split.splits * rows;
+        stats = sums(slots);
+        partials = slots * shape.head_size;
+        scores = tiles == 1 && stats + partials + of_scores * rows <= limit ? of_scores * rows : 0;
+        // (split_of's numbers before they are rounded: as many shares as positions make, within `rounds`, and all rows that a tile has room for)
+        const size_t most_rows = static_cast<long long>(n_q) * shared < kRows ? static_cast<size_t>(n_q) * shared : kRows;
+        size_t most = all_tiles * split.most < split.rounds ? all_tiles * split.most : split.rounds;
+        if (most < all_tiles) most = all_tiles;
+        const size_t shares = sums(most * most_rows) + most * most_rows * shape.head_size, kept = shares + of_scores * most_rows;
+        const size_t with_scores = kept < limit ? kept : limit;
+        bytes = (shares > with_scores ? shares : with_scores) * sizeof(float);
     }
 };
 
@@ -733,7 +747,7 @@ lpp_status lpp_kv4_attention_workspace(const lpp_kv4_shape* shape, int n_heads, 
     LPP_TRY(check("lpp_kv4_attention_workspace", shape, n_heads, n_q));
     LPP_REQUIRE(bytes != nullptr, "lpp_kv4_attention_workspace: null output");
     const int tiles = tiles_of(n_q, n_heads / shape->n_kv_heads);
-    *bytes = Workspace(*shape, n_q, n_heads / shape->n_kv_heads, tiles, split_of(*shape, tiles).splits).bytes();
+    *bytes = Workspace(*shape, n_q, n_heads / shape->n_kv_heads, tiles, split_of(*shape, tiles)).bytes;
     return LPP_OK;
 }
 
@@ -779,7 +793,7 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     // 4000 alike 43 / 41.  Of few heads no more than run at once: 4 sequences of 8000 alike 17 / 23.
     job.per_workgroup = static_cast<float>(shape->n_kv_heads) * job.tiles / (split.waves == 4 ? 1.25f * split.workgroups : split.workgroups);
     job.per_shared = (65536u + job.shared - 1) / job.shared;
-    const Workspace parts(*shape, n_q, job.shared, job.tiles, job.splits);
+    const Workspace parts(*shape, n_q, job.shared, job.tiles, split);
     job.rows = parts.rows;
     job.steps = parts.steps;
     job.stats = static_cast<float2*>(d_workspace);

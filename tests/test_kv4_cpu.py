@@ -170,3 +170,28 @@ def test_oracle_groups():
         y[0, 3] = bad
         assert np.isnan(ko.rounded(y)[0, :32]).all() and not np.isnan(ko.rounded(y)[0, 32:]).any()
     assert not np.isnan(ko.rounded(np.array([[32768.0, -32768.0] * 16], np.float32))).any()
+
+
+def test_a_workspace_of_the_largest_call_serves_smaller_ones(lib):
+    """Bytes do not shrink with sequences, positions, query heads or rows, and stay within partial results of 64 shares of 16 rows."""
+    def need(seqs, kv, room, hs, shared, n_q):
+        n = C.c_size_t()
+        capi.check(lib.lpp_kv4_attention_workspace(Shape(1, seqs, kv, room, hs), kv * shared, n_q, C.byref(n)))
+        tiles = -(-n_q // (16 // shared))
+        assert n.value <= seqs * kv * tiles * 64 * 16 * (hs + 2) * 4
+        return n.value
+
+    rooms = [1, 40, 512, 513, 2000, 3000, 3680, 3681, 6624, 6625, 14000, 14912, 14913, 16000, 27000, 40000, 200000, 1 << 24]
+    rows = [1, 2, 3, 4, 5, 8, 15, 16, 17, 33, 64, 100, 256, 1000, 5000]
+    for hs in (64, 128):
+        for kv in (1, 4, 8):
+            for seqs in (1, 4, 33, 300):
+                table = np.array([[[need(seqs, kv, room, hs, shared, n_q) for n_q in rows if n_q <= room] + [0] * sum(n_q > room for n_q in rows)
+                                   for room in rooms] for shared in range(1, 17)])
+                there = table > 0
+                assert np.all(np.diff(table, axis=0)[there[1:]] >= 0), "query heads"
+                assert np.all(np.diff(table, axis=1)[there[:, :-1]] >= 0), "positions"
+                assert np.all(np.diff(table, axis=2)[there[:, :, 1:]] >= 0), "rows"
+                if seqs > 1:
+                    assert np.all(table >= before), "sequences"
+                before = table

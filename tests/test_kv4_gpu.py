@@ -674,3 +674,23 @@ def test_two_streams_at_once(lib):
         assert np.array_equal(mass[i].to_numpy(np.uint8), mass[2 + i].to_numpy(np.uint8))
     for s in streams:
         hip("hipStreamDestroy", s)
+
+
+@pytest.mark.parametrize("heads,kv,hs,room", [(32, 4, 64, 3000), (8, 2, 128, 7000)])
+def test_one_workspace_for_all_calls(lib, heads, kv, hs, room):
+    """Sized for the most rows a sequence and the whole room, given with its real size to calls of fewer rows and of a smaller cache; nothing behind it
+    is written."""
+    rng = np.random.default_rng(room)
+    need = C.c_size_t()
+    capi.check(lib.lpp_kv4_attention_workspace(Shape(1, 2, kv, room, hs), heads, 16, C.byref(need)))
+    guard = 1 << 16
+    work = DB.from_numpy(np.full(need.value // 4 + guard, np.nan, F))
+    for n_q, positions in ((16, room), (3, room), (2, room), (1, room), (1, 2000), (5, 600), (2, 40)):
+        cache = random_cache(rng, 1, 2, kv, positions, hs)
+        dcache, q = DB.from_numpy(cache.buffer), rng.standard_normal((2, n_q, heads, hs)).astype(F)
+        starts, mass = [positions - n_q, positions // 3], rng.random((1, 2, kv, positions)).astype(F)
+        dq, dout, dst, dmass = DB.from_numpy(q), DB.from_numpy(np.full(q.size, 7.25, F)), ints(starts), DB.from_numpy(mass)
+        capi.check(lib.lpp_kv4_attention(dout.ptr, dq.ptr, dcache.ptr, Shape(1, 2, kv, positions, hs), 0, heads, n_q, dst.ptr, dmass.ptr, work.ptr,
+                                         need.value))
+        check_attention(dout.to_numpy(F).reshape(q.shape), dmass.to_numpy(F).reshape(mass.shape), cache, 0, q, starts, mass)
+    assert np.all(np.isnan(work.to_numpy(F, guard, need.value)))
