@@ -802,11 +802,6 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     const long long groups = static_cast<long long>(job.heads) * job.tiles * job.splits;
     LPP_REQUIRE(groups * dev::kWave * split.waves < (1ll << 32),
                 "lpp_kv4_attention: %u sequences times KV heads and %d rows are too many for a launch", job.heads, n_q);
-    const dim3 grid(static_cast<unsigned>(groups));
-    if (shape->head_size == 64)
-        LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
-    else
-        LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
     const int merges = job.splits > 1 ? (job.tiles * job.rows + kFinishWaves - 1) / kFinishWaves : 0;
     // The positions of one of the account's blocks.  From kept scores of one tile: as many rounds of 1024, up to 8, as leave four blocks to a compute
     // unit.
@@ -817,9 +812,15 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
         span *= each < 1 ? 1 : each < 8 ? static_cast<int>(each) : 8;
     }
     const int accounts = d_mass != nullptr ? (shape->seq_len + span - 1) / span : 0, blocks = merges + accounts;
+    LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32),
+                "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch", job.heads, shape->seq_len);
+    // (nothing is refused from here on)
+    const dim3 grid(static_cast<unsigned>(groups));
+    if (shape->head_size == 64)
+        LPP_TRY(split.waves == 8 ? (launch_attend<64, 8>(job, grid)) : (launch_attend<64, 4>(job, grid)));
+    else
+        LPP_TRY(split.waves == 8 ? (launch_attend<128, 8>(job, grid)) : (launch_attend<128, 4>(job, grid)));
     if (blocks > 0) {
-        LPP_REQUIRE(static_cast<long long>(blocks) * job.heads * kFinishThreads < (1ll << 32),
-                    "lpp_kv4_attention: %u sequences times KV heads of %d positions are too many for a launch", job.heads, shape->seq_len);
         const auto kernel = shape->head_size == 64 ? (kept ? &finish_kernel<64, true> : &finish_kernel<64, false>)
                                                    : (kept ? &finish_kernel<128, true> : &finish_kernel<128, false>);
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks) * job.heads), dim3(kFinishThreads), 0, stream(), job, accounts, span);

@@ -195,3 +195,11 @@ def test_a_workspace_of_the_largest_call_serves_smaller_ones(lib):
                 if seqs > 1:
                     assert np.all(table >= before), "sequences"
                 before = table
+
+
+def test_attention_too_large_for_a_launch_is_refused_before_any(lib):
+    """Positions of so many KV heads that the account's blocks pass a launch: nothing is launched, the attention included."""
+    far = [(i + 1) << 40 for i in range(6)]
+    shape, need = Shape(1, 128, 8, 1 << 20, 64), C.c_size_t()
+    capi.check(lib.lpp_kv4_attention_workspace(shape, 128, 2, C.byref(need)))
+    refused(lib, lib.lpp_kv4_attention(far[0], far[1], far[2], shape, 0, 128, 2, far[3], far[4], far[5], need.value), b"too many for a launch")
