@@ -534,8 +534,8 @@ lpp_status lpp_kv4_attention(float *d_out, const float *d_q, const void *d_cache
  * .. of d_dst, their mass to d_dst_mass, whose further positions up to dst->seq_len are set to zero; rows
  * behind the kept ones stay as they were. d_dst_lengths[s] = min(n, keep).  d_kept: [n_seqs][n_kv_heads][keep],
  * the position each kept row had, -1 behind them. The shapes differ in n_layers and seq_len at most; 0 <=
- * recent <= keep <= dst->seq_len.  d_dst_lengths must not be d_lengths, nor d_dst_mass d_mass: the lengths are
- * the same for every layer, and the next layer's call reads them again. */
+ * recent <= keep <= dst->seq_len.  What is written must not overlap anything else: d_lengths and d_mass, too,
+ * are read again by the next layer's call. */
 lpp_status lpp_kv4_evict(void *d_dst, const lpp_kv4_shape *dst, int dst_layer, float *d_dst_mass, int *d_dst_lengths,
                          int *d_kept, const void *d_src, const lpp_kv4_shape *src, int src_layer, const float *d_mass,
                          const int *d_lengths, int keep, int recent);

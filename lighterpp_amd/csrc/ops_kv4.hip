@@ -467,11 +467,21 @@ lpp_status lpp_kv4_evict(void* d_dst, const lpp_kv4_shape* dst, int dst_layer, f
                 dst->seq_len);
     const long long planes = static_cast<long long>(dst->n_seqs) * dst->n_kv_heads;
     LPP_REQUIRE(planes * kSelectThreads < (1ll << 32), "lpp_kv4_evict: %lld sequences times KV heads", planes);
-    LPP_REQUIRE(!ranges_overlap(d_dst, kv4_bytes(*dst), d_src, kv4_bytes(*src)), "lpp_kv4_evict: the caches overlap");
-    const size_t dst_mass_bytes = kv4_layer_rows(*dst) * dst->n_layers * 4, src_mass_bytes = kv4_layer_rows(*src) * src->n_layers * 4;
-    LPP_REQUIRE(!ranges_overlap(d_dst_mass, dst_mass_bytes, d_mass, src_mass_bytes), "lpp_kv4_evict: d_dst_mass overlaps d_mass");
-    LPP_REQUIRE(!ranges_overlap(d_dst_lengths, 4 * static_cast<size_t>(dst->n_seqs), d_lengths, 4 * static_cast<size_t>(dst->n_seqs)),
-                "lpp_kv4_evict: d_dst_lengths overlaps d_lengths");
+    const struct {
+        const char* name;
+        const void* at;
+        size_t bytes;
+    } buffers[] = {{"d_dst", d_dst, kv4_bytes(*dst)},
+                   {"d_dst_mass", d_dst_mass, kv4_layer_rows(*dst) * dst->n_layers * 4},
+                   {"d_dst_lengths", d_dst_lengths, 4 * static_cast<size_t>(dst->n_seqs)},
+                   {"d_kept", d_kept, 4 * static_cast<size_t>(planes) * keep},
+                   {"d_src", d_src, kv4_bytes(*src)},
+                   {"d_mass", d_mass, kv4_layer_rows(*src) * src->n_layers * 4},
+                   {"d_lengths", d_lengths, 4 * static_cast<size_t>(src->n_seqs)}};
+    for (int a = 0; a < 4; ++a)  // (what is written, and all behind it)
+        for (int b = a + 1; b < 7; ++b)
+            LPP_REQUIRE(!ranges_overlap(buffers[a].at, buffers[a].bytes, buffers[b].at, buffers[b].bytes), "lpp_kv4_evict: %s overlaps %s", buffers[a].name,
+                        buffers[b].name);
     float* dst_mass = d_dst_mass + kv4_layer_rows(*dst) * dst_layer;
     const float* src_mass = d_mass + kv4_layer_rows(*src) * src_layer;
     const auto select = src->seq_len <= 4 * kSelectThreads    ? &select_kernel<4, true>

@@ -203,3 +203,16 @@ def test_attention_too_large_for_a_launch_is_refused_before_any(lib):
     shape, need = Shape(1, 128, 8, 1 << 20, 64), C.c_size_t()
     capi.check(lib.lpp_kv4_attention_workspace(shape, 128, 2, C.byref(need)))
     refused(lib, lib.lpp_kv4_attention(far[0], far[1], far[2], shape, 0, 128, 2, far[3], far[4], far[5], need.value), b"too many for a launch")
+
+
+def test_evict_refuses_every_overlap(lib):
+    """Each of the four buffers that are written with each other and with each of the three that are read."""
+    src, dst = Shape(2, 3, 2, 100, 64), Shape(2, 3, 2, 20, 64)
+    sizes = [2 * 3 * 2 * 20 * 80, 2 * 3 * 2 * 20 * 4, 3 * 4, 3 * 2 * 20 * 4, 2 * 3 * 2 * 100 * 80, 2 * 3 * 2 * 100 * 4, 3 * 4]
+    for a in range(4):
+        for b in range(7):
+            if a == b:
+                continue
+            at = [(i + 1) * P for i in range(7)]
+            at[a] = (at[b] + sizes[b] - 1) // 16 * 16  # begins in b's last bytes
+            refused(lib, lib.lpp_kv4_evict(at[0], dst, 1, at[1], at[2], at[3], at[4], src, 1, at[5], at[6], 20, 5), b"overlaps")
