@@ -418,6 +418,10 @@ lpp_status lpp_kv4_store(void* d_cache, const lpp_kv4_shape* shape, int layer, c
     const size_t in_bytes = (static_cast<size_t>(n_tokens - 1) * kv_stride + kv_dim) * (type == LPP_F32 ? 4 : 2);
     LPP_REQUIRE(!ranges_overlap(d_k, in_bytes, d_cache, kv4_bytes(*shape)) && !ranges_overlap(d_v, in_bytes, d_cache, kv4_bytes(*shape)),
                 "lpp_kv4_store: the rows overlap the cache");
+    const size_t seqs_bytes = static_cast<size_t>(shape->n_seqs) * 4;
+    LPP_REQUIRE((d_offsets == nullptr || !ranges_overlap(d_offsets, seqs_bytes + 4, d_cache, kv4_bytes(*shape))) &&
+                    (d_starts == nullptr || !ranges_overlap(d_starts, seqs_bytes, d_cache, kv4_bytes(*shape))),
+                "lpp_kv4_store: d_offsets or d_starts overlaps the cache");
     const Kv4Layer to = kv4_layer(d_cache, *shape, layer);
     const dim3 grid((static_cast<unsigned>(n_tokens) + kStoreThreads / dev::kWave - 1) / (kStoreThreads / dev::kWave));
     if (type == LPP_F32)

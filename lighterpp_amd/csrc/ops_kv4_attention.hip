@@ -772,6 +772,11 @@ lpp_status lpp_kv4_attention(float* d_out, const float* d_q, const void* d_cache
     LPP_REQUIRE(mass_bytes == 0 || (!ranges_overlap(d_mass, mass_bytes, d_workspace, need) && !ranges_overlap(d_mass, mass_bytes, d_q, rows_bytes) &&
                                     !ranges_overlap(d_mass, mass_bytes, d_out, rows_bytes) && !ranges_overlap(d_mass, mass_bytes, d_cache, kv4_bytes(*shape))),
                 "lpp_kv4_attention: d_mass overlaps the workspace, q, out or the cache");
+    LPP_REQUIRE(!ranges_overlap(d_out, rows_bytes, d_cache, kv4_bytes(*shape)), "lpp_kv4_attention: d_out overlaps the cache");
+    const size_t starts_bytes = static_cast<size_t>(shape->n_seqs) * 4;
+    LPP_REQUIRE(!ranges_overlap(d_starts, starts_bytes, d_out, rows_bytes) && !ranges_overlap(d_starts, starts_bytes, d_workspace, need) &&
+                    (mass_bytes == 0 || !ranges_overlap(d_starts, starts_bytes, d_mass, mass_bytes)),
+                "lpp_kv4_attention: d_starts overlaps out, the workspace or d_mass");
     AttendJob job;
     job.out = d_out;
     job.q = d_q;

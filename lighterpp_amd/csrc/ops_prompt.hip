@@ -535,7 +535,8 @@ lpp_status lpp_prompt_attention(void* d_out, const void* d_q, const lpp_half* d_
     const auto bytes = [&](int stride, long long row, int of) { return (static_cast<size_t>(n_tokens - 1) * stride + row) * of; };
     const size_t out_bytes = bytes(out_stride, width, size), q_bytes = bytes(q_stride, width, size), kv_bytes = bytes(kv_stride, kv_width, 2);
     LPP_REQUIRE(!ranges_overlap(d_out, out_bytes, d_q, q_bytes) && !ranges_overlap(d_out, out_bytes, d_k, kv_bytes) &&
-                    !ranges_overlap(d_out, out_bytes, d_v, kv_bytes),
+                    !ranges_overlap(d_out, out_bytes, d_v, kv_bytes) &&
+                    (d_offsets == nullptr || !ranges_overlap(d_out, out_bytes, d_offsets, (static_cast<size_t>(n_seqs) + 1) * 4)),
                 "lpp_prompt_attention: d_out overlaps an input");
     PromptJob job;
     job.out = d_out;

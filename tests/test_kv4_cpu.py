@@ -216,3 +216,18 @@ def test_evict_refuses_every_overlap(lib):
             at = [(i + 1) * P for i in range(7)]
             at[a] = (at[b] + sizes[b] - 1) // 16 * 16  # begins in b's last bytes
             refused(lib, lib.lpp_kv4_evict(at[0], dst, 1, at[1], at[2], at[3], at[4], src, 1, at[5], at[6], 20, 5), b"overlaps")
+
+
+def test_outputs_over_the_cache_or_the_ints_are_refused(lib):
+    s, need = Shape(1, 3, 2, 10, 64), C.c_size_t()
+    capi.check(lib.lpp_kv4_attention_workspace(s, 8, 2, C.byref(need)))
+    attend = lambda out=P, cache=3 * P, starts=6 * P, mass=5 * P: \
+        lib.lpp_kv4_attention(out, 2 * P, cache, s, 0, 8, 2, starts, mass, 4 * P, need.value)  # noqa: E731
+    refused(lib, attend(out=3 * P + 4784), b"d_out overlaps the cache")
+    for base in (P, 4 * P, 5 * P):
+        refused(lib, attend(starts=base + 8), b"d_starts overlaps")
+    refused(lib, attend(starts=P - 8), b"d_starts overlaps")
+    store = lambda offsets=None, starts=None: lib.lpp_kv4_store(P, s, 0, 2 * P, 3 * P, 0, 128, offsets, 6, starts)  # noqa: E731
+    refused(lib, store(offsets=P - 12), b"overlaps the cache")
+    refused(lib, store(starts=P + 4796), b"overlaps the cache")
+    refused(lib, lib.lpp_prompt_attention(P, 2 * P, 3 * P, 4 * P, 0, P - 8, 2, 8, 4, 2, 64, 256, 128, 256), b"overlaps")
