@@ -498,11 +498,11 @@ typedef struct lpp_kv4_shape {
 } lpp_kv4_shape;
 lpp_status lpp_kv4_bytes(const lpp_kv4_shape *shape, size_t *bytes);
 
-/* Rows of K and V into one layer of the cache.  k and v: [n_tokens][n_kv_heads * head_size] of `type`, rows at
- * multiples of 16 bytes, kv_stride elements apart; they and the ints must not overlap the cache.  Rows
- * d_offsets[s] .. d_offsets[s + 1] - 1 are sequence s's, as above; NULL: n_tokens / n_seqs rows each.  The j-th
- * of them goes to position d_starts[s] + j (d_starts NULL: j); a row whose position is not within 0 .. seq_len
- * - 1 is dropped, so a start of -n for n rows skips a sequence. */
+/* Rows of K and V into one layer of the cache, fewer than 2^26 - 3 at a time.  k and v: [n_tokens][n_kv_heads *
+ * head_size] of `type`, rows at multiples of 16 bytes, kv_stride elements apart; they and the ints must not
+ * overlap the cache.  Rows d_offsets[s] .. d_offsets[s + 1] - 1 are sequence s's, as above; NULL: n_tokens /
+ * n_seqs rows each.  The j-th of them goes to position d_starts[s] + j (d_starts NULL: j); a row whose position
+ * is not within 0 .. seq_len - 1 is dropped, so a start of -n for n rows skips a sequence. */
 lpp_status lpp_kv4_store(void *d_cache, const lpp_kv4_shape *shape, int layer, const void *d_k, const void *d_v, int type,
                          int kv_stride, const int *d_offsets, int n_tokens, const int *d_starts);
 
@@ -514,9 +514,9 @@ lpp_status lpp_kv4_load(lpp_half *d_k, lpp_half *d_v, const void *d_cache, const
 
 /* Attention of n_q new rows a sequence over one layer of the cache, which holds them already: row j attends to
  * positions 0 .. d_starts[s] + j, with the d_starts that the store was given (cut to the positions there are; a
- * row that attends to none gives zeros).  q and out: fp32 [n_seqs][n_q][n_heads * head_size], 16-byte aligned,
- * a query beyond +-65504 gives NaN.  out, mass and workspace must not overlap each other or what is read.  n_q =
- * 1 is a decode step.
+ * row that attends to none gives zeros); at most 65535 sequences and as many KV heads.  q and out: fp32
+ * [n_seqs][n_q][n_heads * head_size], 16-byte aligned, a query beyond +-65504 gives NaN.  out, mass and workspace
+ * must not overlap each other or what is read.  n_q = 1 is a decode step.
  * d_mass (may be NULL): fp32 [n_layers][n_seqs][n_kv_heads][seq_len]; to every position is added the weight it
  * got, summed over the rows and the query heads of its KV head.  Set it to zero when a sequence begins.
  * d_workspace: lpp_kv4_attention_workspace() bytes, 16-byte aligned, apart from all else; it need not be set to

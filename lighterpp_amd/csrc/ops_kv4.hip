@@ -411,6 +411,8 @@ lpp_status lpp_kv4_store(void* d_cache, const lpp_kv4_shape* shape, int layer, c
     const long long kv_dim = static_cast<long long>(shape->n_kv_heads) * shape->head_size;
     LPP_REQUIRE(kv_stride >= kv_dim, "lpp_kv4_store: kv_stride = %d is less than a row of %lld", kv_stride, kv_dim);
     if (n_tokens == 0) return LPP_OK;
+    const unsigned blocks = (static_cast<unsigned>(n_tokens) + kStoreThreads / dev::kWave - 1) / (kStoreThreads / dev::kWave);
+    LPP_REQUIRE(static_cast<long long>(blocks) * kStoreThreads < (1ll << 32), "lpp_kv4_store: n_tokens = %d are too many for a launch", n_tokens);
     LPP_REQUIRE(d_k && d_v, "lpp_kv4_store: null pointer");
     const int per16 = type == LPP_F32 ? 4 : 8;
     LPP_REQUIRE(reinterpret_cast<uintptr_t>(d_k) % 16 == 0 && reinterpret_cast<uintptr_t>(d_v) % 16 == 0 && kv_stride % per16 == 0,
@@ -423,7 +425,7 @@ lpp_status lpp_kv4_store(void* d_cache, const lpp_kv4_shape* shape, int layer, c
                     (d_starts == nullptr || !ranges_overlap(d_starts, seqs_bytes, d_cache, kv4_bytes(*shape))),
                 "lpp_kv4_store: d_offsets or d_starts overlaps the cache");
     const Kv4Layer to = kv4_layer(d_cache, *shape, layer);
-    const dim3 grid((static_cast<unsigned>(n_tokens) + kStoreThreads / dev::kWave - 1) / (kStoreThreads / dev::kWave));
+    const dim3 grid(blocks);
     if (type == LPP_F32)
         hipLaunchKernelGGL((store_kernel<float>), grid, dim3(kStoreThreads), 0, stream(), to, static_cast<const float*>(d_k), static_cast<const float*>(d_v),
                            kv_stride, d_offsets, d_starts, n_tokens, shape->n_seqs, shape->n_kv_heads, shape->head_size, shape->seq_len);

@@ -231,3 +231,9 @@ def test_outputs_over_the_cache_or_the_ints_are_refused(lib):
     refused(lib, store(offsets=P - 12), b"overlaps the cache")
     refused(lib, store(starts=P + 4796), b"overlaps the cache")
     refused(lib, lib.lpp_prompt_attention(P, 2 * P, 3 * P, 4 * P, 0, P - 8, 2, 8, 4, 2, 64, 256, 128, 256), b"overlaps")
+
+
+def test_store_too_large_for_a_launch(lib):
+    s, far = Shape(1, 1, 1, 1 << 24, 64), [(i + 1) << 40 for i in range(3)]
+    for n in (1 << 26, (1 << 26) - 3, 2 ** 31 - 1):
+        refused(lib, lib.lpp_kv4_store(far[0], s, 0, far[1], far[2], capi.F16, 64, None, n, None), b"too many for a launch")
