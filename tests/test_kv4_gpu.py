@@ -694,3 +694,56 @@ def test_one_workspace_for_all_calls(lib, heads, kv, hs, room):
                                          need.value))
         check_attention(dout.to_numpy(F).reshape(q.shape), dmass.to_numpy(F).reshape(mass.shape), cache, 0, q, starts, mass)
     assert np.all(np.isnan(work.to_numpy(F, guard, need.value)))
+
+
+def part_of(cache, seqs):
+    """Some of a cache's sequences."""
+    part = ko.Cache(cache.dims[0], len(seqs), *cache.dims[2:], cache.hs)
+    for w in range(2):
+        part.codes[w][:], part.scales[w][:] = cache.codes[w][:, seqs], cache.scales[w][:, seqs]
+    return part
+
+
+@pytest.mark.parametrize("seqs,heads,kv,hs,room,n_q", [(9, 16, 8, 128, 5000, 1), (9, 32, 4, 128, 3001, 5), (17, 8, 4, 64, 2500, 1)])
+def test_many_heads_and_several_shares(lib, seqs, heads, kv, hs, room, n_q):
+    """Four wavefronts to a share, positions enough for several, with and without the account, whose scores are kept (one tile of rows) or made again."""
+    rng = np.random.default_rng(room)
+    lengths = np.concatenate([[room, n_q, 0], rng.integers(room // 6, room, seqs - 3)])
+    cache = random_cache(rng, 1, seqs, kv, room, hs)
+    dcache, q = DB.from_numpy(cache.buffer), rng.standard_normal((seqs, n_q, heads, hs)).astype(F)
+    mass, starts = rng.random((1, seqs, kv, room)).astype(F), lengths - n_q
+    got, got_mass = attend(lib, dcache, cache, 0, q, starts, mass)
+    check_attention(got, got_mass, cache, 0, q, starts, mass)
+    assert np.array_equal(attend(lib, dcache, cache, 0, q, starts)[0], got)
+
+
+def test_account_of_many_heads_from_kept_scores(lib):
+    """So many sequences that a block of the account takes several rounds of 1024 positions: a sample of them."""
+    rng = np.random.default_rng(21)
+    seqs, heads, kv, hs, room = 128, 16, 8, 64, 1100
+    cache = random_cache(rng, 1, seqs, kv, room, hs)
+    q, mass = rng.standard_normal((seqs, 1, heads, hs)).astype(F), rng.random((1, seqs, kv, room)).astype(F)
+    starts = rng.integers(0, room, seqs)
+    starts[[0, 1, 50, 127]] = [room - 1, 1023, 1024, 1026]
+    got, got_mass = attend(lib, DB.from_numpy(cache.buffer), cache, 0, q, starts, mass)
+    some = [0, 1, 2, 3, 50, 90, 126, 127]
+    check_attention(got[some], got_mass[:, some], part_of(cache, some), 0, q[some], starts[some], mass[:, some])
+    for s in range(seqs):
+        assert np.array_equal(got_mass[0, s, :, starts[s] + 1:], mass[0, s, :, starts[s] + 1:])
+        added = got_mass[0, s].astype(np.float64).sum(-1) - mass[0, s].astype(np.float64).sum(-1)
+        # (the weights of two heads; every position's total is below 4, so its rounding is 2^-23 at most, and its weights' errors are far below 2^-16)
+        assert np.all(np.abs(added - 2) <= room * 2.0 ** -23 + 2 * 2.0 ** -16)
+
+
+@pytest.mark.parametrize("heads,hs,room", [(4, 64, 5001), (4, 128, 8000)])
+def test_account_made_again_for_several_rows_of_one_tile(lib, heads, hs, room):
+    """Four rows of four heads, one tile, of more positions than whose scores are kept (16 rows: 4 bytes each of all positions and the partial results of a
+    share for every 512 of them are more than those of 64 shares)."""
+    assert 16 * room + -(-room // 512) * 16 * (hs + 2) > 64 * 16 * (hs + 2)
+    rng = np.random.default_rng(room)
+    lengths = [room - 1, 900, 4, 2]
+    cache = random_cache(rng, 1, len(lengths), 1, room, hs)
+    q, mass = rng.standard_normal((len(lengths), 4, heads, hs)).astype(F), rng.random((1, len(lengths), 1, room)).astype(F)
+    starts = [n - 4 for n in lengths]
+    got, got_mass = attend(lib, DB.from_numpy(cache.buffer), cache, 0, q, starts, mass)
+    check_attention(got, got_mass, cache, 0, q, starts, mass)

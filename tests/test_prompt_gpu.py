@@ -284,3 +284,68 @@ def test_binary16_is_rounded_once(lib, heads, kv, hs, lengths):
         tol += (np.abs(want) + tol) * 2.0 ** -11 + 2.0 ** -25
         off = np.abs(got[a:b][rows] - want)
         assert np.all(off <= tol), (a, b, float((off / tol).max()))
+
+
+def rows_of_shape(lib, shape, heads, kv, hs):
+    """Rows in all for which the library takes workgroups of 1 x 4, 2 x 2 or 4 x 1 wavefronts (by the tiles of 32 rows there are)."""
+    units = C.c_int()
+    capi.check(lib.lpp_device_info(None, 0, C.byref(units), None))
+    few, many = (2 if hs == 64 else 1) * units.value, 6 * units.value
+    tiles = {"1x4": few // 2, "2x2": few + units.value // 2, "4x1": many + units.value // 2}[shape]
+    rows = tiles // kv * 32 // (heads // kv)
+    assert {"1x4": lambda t: t <= few, "2x2": lambda t: few < t <= many, "4x1": lambda t: t > many}[shape]((rows * (heads // kv) + 31) // 32 * kv)
+    return rows
+
+
+def ragged(rows):
+    """Ends inside a tile, a single row, an empty sequence, and a long one."""
+    lengths = [1, 37, 0, rows // 5, rows // 7 + 3]
+    return lengths + [rows - sum(lengths)]
+
+
+SHAPES = [(24, 8, 64), (32, 8, 64), (30, 6, 128), (32, 8, 128)]
+
+
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("heads,kv,hs", SHAPES)
+@pytest.mark.parametrize("shape", ["2x2", "4x1"])
+def test_workgroups_of_every_shape(lib, shape, heads, kv, hs, typ):
+    """Rows enough for the workgroups that several rows of wavefronts share: a sample of every sequence's rows against the oracle."""
+    lengths = ragged(rows_of_shape(lib, shape, heads, kv, hs))
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    q, k, v = inputs(heads * hs + len(shape), int(offsets[-1]), heads, kv, hs, typ)
+    got = run(lib, q, k, v, offsets, pad=1)
+    for a, b in zip(offsets[:-1], offsets[1:]):
+        rows = np.unique(np.clip([0, 1, 31, 32, 62, 63, 64, 127, 128, b - a - 33, b - a - 2, b - a - 1] + list(np.linspace(0, b - a - 1, 9).astype(int)), 0, b - a - 1))
+        if a == b:
+            continue
+        want, _, tol = ko.attend_tolerance(q[a:b][rows], k[a:b].transpose(1, 0, 2), v[a:b].transpose(1, 0, 2), [int(j) + 1 for j in rows],
+                                           binary16=typ is H)
+        off = np.abs(got[a:b][rows].astype(np.float64) - want)
+        assert np.all(off <= tol), (a, b, float((off / tol).max()))
+
+
+@pytest.mark.parametrize("typ", [F, H])
+@pytest.mark.parametrize("heads,kv,hs", SHAPES)
+@pytest.mark.parametrize("shape", ["2x2", "4x1"])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_nothing_from_other_rows_in_every_shape(lib, where, shape, heads, kv, hs, typ):
+    """As above with few rows: NaN rows in the middle and at ends do not reach the rows before them or other sequences, bit for bit."""
+    lengths = ragged(rows_of_shape(lib, shape, heads, kv, hs))
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    total = int(offsets[-1])
+    q, k, v = inputs(heads + hs, total, heads, kv, hs, typ)
+    clean = run(lib, q, k, v, offsets)
+    x = {"k": k.copy(), "v": v.copy()}
+    seen = np.zeros(total, bool)
+    for s, at in ((1, 36), (3, lengths[3] - 1), (4, lengths[4] // 2), (5, lengths[5] * 2 // 3)):
+        x[where][offsets[s] + at, :, 3] = np.nan
+        seen[offsets[s] + at:offsets[s + 1]] = True
+    got = run(lib, q, x["k"], x["v"], offsets)
+    assert np.array_equal(got[~seen], clean[~seen])
+    if where == "k":
+        assert np.isnan(got[seen]).all()
+    else:
+        assert np.isnan(got[seen][:, :, 3]).all()
+        other = np.arange(hs) != 3
+        assert np.array_equal(got[seen][:, :, other], clean[seen][:, :, other])
