@@ -101,6 +101,23 @@ struct Kv4Reader {
     }
 };
 
+// v + that of the same lane of the wavefront's other half.
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Sum over the wavefront's lanes up to and with this one.
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr by 1, 2, 4, 8: zero comes in
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
+    const int row = lane_id() >> 4;
+    return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
+}
+
 // How many of n values that do not decrease, value(0) .. value(n - 1), are at or below `limit`.  The whole wavefront looks at 64 of them at a time:
 // one round for up to 64, two for 4096.
 template <typename Value>

@@ -192,17 +192,6 @@ __device__ __forceinline__ uint32_t key_of(float mass) {
     return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// Sum over the wavefront's lanes up to and with this one.
-__device__ __forceinline__ int wave_inclusive_sum(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr by 1, 2, 4, 8: zero comes in
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
-    const int row = lane_id() >> 4;
-    return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
-}
-
 // One workgroup per sequence and KV head: the keep - recent positions of largest weight among the first n - recent, then the list in order. The
 // smallest weight kept is found by its bits, 11, 11 and 10 at a time from the top: counts of every value of those bits among the weights that agree
 // with what is known, added up from above.  A thread holds kHeld weights in registers (kOnce: all it has; else stretches of them, read again in every

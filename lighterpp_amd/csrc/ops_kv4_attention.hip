@@ -20,7 +20,6 @@ namespace {
 
 using namespace dev;
 
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 16;       // of a tile: (16 / shared) new rows x the query heads of a KV head
@@ -60,10 +59,6 @@ struct AttendJob {
     }
 };
 
-__device__ __forceinline__ float halves_sum(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 __device__ __forceinline__ float rows_max(float v) {
     const unsigned u = __float_as_uint(v);
     const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -252,8 +247,9 @@ __global__ __launch_bounds__(kWave * kWaves, kHs == 64 ? 4 : 3) void attend_kern
     float minus_one = -1.0f;
     asm("" : "+v"(minus_one));
 
-    // V rows of a step, in this wavefront's own LDS: 16-byte pieces in an order that keeps writes and transposing reads free of bank
-    // conflicts
+    // V rows of a step, in this wavefront's own LDS: 16-byte pieces in an order that keeps writes free of bank conflicts, and transposing reads of
+    // heads of 64.  (Of heads of 128 half a wavefront reads a pair of pieces of eight rows, and rows four apart have theirs in the same banks: two cycles
+    // for one, 41 % of the LDS's in a batch of 32 sequences.)
     char* values = lds + wave * kWaveBytes;
     auto swizzle = [](int row) { return kHs == 64 ? 2 * ((row >> 1) & 3) : 4 * (row & 3) + ((row >> 2) & 3); };
     int v_at[kDTiles], v_to[kWords];  // (of the first sixteen positions; the others are 16 rows further, in the same order)

@@ -60,24 +60,10 @@ __device__ __forceinline__ float halves_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ float halves_sum(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 template <int kCount>
 __device__ __forceinline__ void wait_requests() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCount) : "memory");
 }
-__device__ __forceinline__ int wave_inclusive_sum(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr by 1, 2, 4, 8: zero comes in
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-    const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = r0 + __builtin_amdgcn_readlane(v, 31), r2 = r1 + __builtin_amdgcn_readlane(v, 47);
-    const int row = lane_id() >> 4;
-    return v + (row == 0 ? 0 : row == 1 ? r0 : row == 2 ? r1 : r2);
-}
-
 __device__ __forceinline__ int wave_sum_int(int v) { return __builtin_amdgcn_readlane(wave_inclusive_sum(v), kWave - 1); }
 
 // The workgroup's tile: which of its sequence's tiles it is, and the sequence's rows (returned; 0: it has none).  Up to 64 sequences: in the order of

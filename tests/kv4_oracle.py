@@ -110,7 +110,7 @@ def score_error(q, k, ends):
 def attend_tolerance(q, k, v, ends, binary16=False):
     """[rows, heads, hs]: a weight's relative error is twice the scores' (its own and that of the sum it is divided by), and 2^-20 for the
     exponential, the remainder's rounding (2^-22) and the quotient; the sums of n terms in fp32 add n 2^-24 at most, twice.
-    binary16: the weights are rounded where they meet V (2^-11, or 2^-25 of the largest where they are subnormal), and the output is."""
+    binary16: the output is rounded (2^-11, or 2^-25 where it is subnormal), and there is room for weights of as many bits."""
     rows, heads, hs = q.shape
     kv_heads = k.shape[0]
     d = score_error(q, k, ends)
@@ -125,7 +125,7 @@ def attend_tolerance(q, k, v, ends, binary16=False):
             part = weights[j, h, :e] @ a
             tol[j, h] = part * (2 * d[j, h] + 2.0 ** -20 + 2 * e * 2.0 ** -24)
             if binary16:
-                # (the sum is of the unrounded weights; its own share of the largest weight, 1 / n at least, is what the subnormals' step is relative to)
+                # (of weights of 11 bits and a sum of unrounded ones; the kernels keep the remainders, and test_prompt_gpu.py has the bound for that)
                 tol[j, h] += part * 2.0 ** -11 + a.sum(0) * 2.0 ** -25 * weights[j, h].max() + np.abs(out[j, h]) * 2.0 ** -11 + 2.0 ** -25
     return out, weights, tol
 

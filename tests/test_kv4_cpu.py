@@ -237,3 +237,20 @@ def test_store_too_large_for_a_launch(lib):
     s, far = Shape(1, 1, 1, 1 << 24, 64), [(i + 1) << 40 for i in range(3)]
     for n in (1 << 26, (1 << 26) - 3, 2 ** 31 - 1):
         refused(lib, lib.lpp_kv4_store(far[0], s, 0, far[1], far[2], capi.F16, 64, None, n, None), b"too many for a launch")
+
+
+def test_scale_against_the_quotient_in_64_bits():
+    """The format's scale, the range times the fp32 number 1/15, is the fifteenth of the range to its own rounding (2^-11, or 2^-25 where it is subnormal) and three
+    of fp32: the difference, 1/15, the product.  Every value stands for one within half a step of it."""
+    rng = np.random.default_rng(13)
+    x = (rng.standard_normal((20000, 32)) * np.exp(3 * rng.standard_normal((20000, 1)))).astype(np.float32)
+    x[:2000] *= np.float32(1e-6)
+    x = np.clip(x, -32768, 32768)
+    _, scale, low = ko.quantise(x)
+    g = x.astype(np.float64)
+    span = g.max(-1) - g.min(-1)
+    assert np.all(np.abs(scale[:, 0].astype(np.float64) - span / 15) <= span / 15 * (2.0 ** -11 + 3.01 * 2.0 ** -24) + 2.0 ** -25)
+    got = ko.rounded(x).astype(np.float64)
+    # half a step, fifteen times the scale's rounding, and the roundings of lowest and value
+    bound = span / 30 + span * 2.0 ** -11 * 1.01 + 2 * np.abs(g).max(-1) * 2.0 ** -11 * 1.01 + 17 * 2.0 ** -25
+    assert np.all(np.abs(got - g) <= bound[:, None])
