@@ -45,8 +45,10 @@ struct AttendJob {
     __device__ __forceinline__ int end_of(int start, int row) const { return min(max(start + row + 1, 0), seq_len); }
     __device__ __forceinline__ int tokens() const { return static_cast<int>(kRows * per_shared >> 16); }  // of a tile
     // How many shares a sequence's `positions` are cut into: of all sequences' positions, as many to each as gives `workgroups` of them in all,
-    // but no fewer than `least`.  (All lanes call it and read the sequences' starts, 64 at a time; the same sum in every workgroup.  Of very many
-    // sequences all are taken to be as long as this one.)
+    // but no fewer than `least`.  (All lanes call it and read the sequences' starts, 64 at a time; the same sum in every workgroup.  Of more than
+    // 256 sequences all are taken to be as long as this one, which leaves one that is much longer than the others too few shares: with 300, one of 30000
+    // positions and the others of 30, 8 KV heads of 64, 176 us for 75 with the sum.  Any others pay for the sum: 300 of 30 positions 33 us for 22, of 1000
+    // 64 for 52; 1000 of up to 2000 238 for 158; 4000 1129 for 555.)
     __device__ __forceinline__ int shares_of(int positions) const {
         float all = n_seqs > 4 * kWave ? static_cast<float>(positions) * n_seqs : 0.0f;
         if (n_seqs <= 4 * kWave)

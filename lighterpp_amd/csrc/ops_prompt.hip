@@ -13,11 +13,12 @@
 // its own rounding makes 2.0e-4; with the remainders it is rounded once, and is within 2e-5 of fp32 arithmetic rounded.  They cost 4 % with prompts of
 // 250 rows, a fifth at 2000 and a third at 8191.)
 //
-// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 731 us, 1130 TFLOP/s of products, where a matrix product of 8192^3
-// reaches 1186: matrix cores at the clock that the power leaves.  Without exponentials, a maximum, or the multiplication by the scale fp32 gained 0 to 10 %;
-// two query tiles to a wavefront, for half the reads of LDS, are slower (half the wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of
-// 128 do not fit the registers).  Several pages (7 of up to 1500 rows, 32 heads of 64 on 8, fp32): 111 us, of which the remainders' products are a third.  Few rows (4 of up to 45): 5.9 us, the
-// time of the requests one after the other: offsets, rows, and the write.
+// What bounds it.  A long document (8191 rows, 32 heads of 128 on 8, binary16): 731 to 759 us (machines hold different clocks), 1090 to 1130 TFLOP/s
+// of products, where a matrix product of 8192^3 reaches 1186; matrix cores busy 64 % of the cycles, vector ALUs 50 %, LDS 22 %, at the clock of 1.7
+// GHz that the power leaves.  Without exponentials, a maximum, or the multiplication by the scale fp32 gained 0 to 10 %; two query tiles to a
+// wavefront, for half the reads of LDS, are slower (half the wavefronts: 4096 rows, 32 heads of 64, fp32 224 us for 157; heads of 128 do not fit the
+// registers).  Several pages (7 of up to 1500 rows, 32 heads of 64 on 8, fp32): 111 us, of which the remainders' products are a third.  Few rows (4
+// of up to 45): 5.9 us, the time of the requests one after the other: offsets, rows, and the write.
 #include <type_traits>
 
 #include "kv4.hpp"
@@ -464,7 +465,8 @@ lpp_status launch_as(const PromptJob& job, int n_seqs) {
         LPP_TRY(tell_lds(reinterpret_cast<const void*>(kernel), kLds, sized));
     }
     // (as many tile numbers as find_tile gives to sequences of any lengths: one more than whole tiles for each sequence, and up to kWave of them only
-    // for those that have rows)
+    // for those that have rows.  A number without a tile costs a workgroup that finds out: one prompt of 300 rows, 32 heads of 64 on 8, fp32, among 300
+    // sequences 10.3 us, among 5000 100, by itself 8.3.)
     const int tokens = kR * (32 / job.shared);
     const long long tiles = job.n_tokens / tokens + (n_seqs <= dev::kWave && n_seqs > job.n_tokens ? job.n_tokens : n_seqs);
     const long long blocks = tiles * job.n_kv_heads;
